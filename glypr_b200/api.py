@@ -45,8 +45,13 @@ EXPORTED_SYMBOLS = (
     "glp_tokenizer_info", "glp_tokenize", "glp_tokenize_batch", "glp_format_query", "glp_format_document",
     "glp_task_format", "glp_embed_texts", "glp_engine_embed_text", "glp_embed_tokens_sharded",
     "glp_kernel_status", "glp_status_text", "glp_selftest_wait_timeout", "glp_gate_up_geglu",
-    "glp_qkv_norm_rope",
+    "glp_qkv_norm_rope", "glp_norm_residual_q8", "glp_quantize_rows", "glp_linear",
 )
+
+# element types and activations of glp_norm_residual_q8 / glp_quantize_rows / glp_linear
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "i8": 3, "e4m3": 4}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3, "gelu_erf": 4}
+GLP_QUANT_MAX_H = 32768
 
 # sequence forms of a text (include/glypr_cuda.h GLP_TOKENS_*)
 GLP_TOKENS_BARE = 0      # the BPE ids alone
@@ -81,6 +86,24 @@ class GlpModelInfo(ctypes.Structure):
 
 class GlpTiming(ctypes.Structure):
     _fields_ = [("n_devices", ctypes.c_int), ("device_ms", ctypes.c_float * GLP_MAX_DEVICES)]
+
+
+class GlpNormQ8Args(ctypes.Structure):
+    _fields_ = ([("M", ctypes.c_int), ("H", ctypes.c_int), ("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64),
+                 ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64), ("post_gain", ctypes.c_void_p),
+                 ("gain", ctypes.c_void_p), ("eps", ctypes.c_float), ("layer_scalar", ctypes.c_float),
+                 ("h", ctypes.c_void_p), ("ld_h", ctypes.c_int64), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_int64),
+                 ("scale", ctypes.c_void_p)]
+                + [(n, ctypes.c_int) for n in ("x_dtype", "h_dtype", "q_dtype")])
+
+
+class GlpLinearArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int) for n in ("M", "N", "K", "dtype")]
+                + [("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64), ("w", ctypes.c_void_p),
+                   ("w_up", ctypes.c_void_p), ("ld_w", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("x_scale", "w_scale", "w_up_scale", "bias", "bias_up", "residual")]
+                + [("ld_residual", ctypes.c_int64), ("y", ctypes.c_void_p), ("ld_y", ctypes.c_int64),
+                   ("out_dtype", ctypes.c_int), ("activation", ctypes.c_int)])
 
 
 class GlpProfile(ctypes.Structure):
@@ -158,6 +181,9 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
         L.glp_selftest_wait_timeout.argtypes = [I, I]
         L.glp_gate_up_geglu.argtypes = [P, P, I, I, P, I, P, P]
         L.glp_qkv_norm_rope.argtypes = [P, I, I, I, P, I, P, P, P, ctypes.c_double, I, ctypes.c_float, P, P]
+        L.glp_norm_residual_q8.argtypes = [P, P]
+        L.glp_quantize_rows.argtypes = [P, I, I64, I, I, P, I, I64, P, P]
+        L.glp_linear.argtypes = [P, P]
         _lib = L
         return L
 
@@ -444,6 +470,35 @@ def qkv_norm_rope(d_w: int, n_q_heads: int, n_kv_heads: int, k: int, d_x: int, m
                                            ctypes.c_void_p(d_q_gain), ctypes.c_void_p(d_k_gain),
                                            ctypes.c_void_p(d_pos), float(theta), max_pos, float(eps),
                                            ctypes.c_void_p(d_out), ctypes.c_void_p(stream)))
+
+
+def norm_residual_q8(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dtype: int, d_scale: int, *,
+                     gain: int = 0, post_gain: int = 0, residual: int = 0, h: int = 0, h_dtype: int = DTYPES["bf16"],
+                     eps: float = 1e-6, layer_scalar: float = 1.0, ld_x: int = 0, ld_residual: int = 0, ld_h: int = 0,
+                     ld_q: int = 0, stream: int = 0) -> None:
+    """glp_norm_residual_q8: h = (residual + x~) * layer_scalar and the 8-bit form of RMSNorm(h) * gain.
+    Device pointers as ints (0 = not given), types from ``DTYPES``, pitches in elements (0 = packed)."""
+    a = GlpNormQ8Args(m, h_len, d_x, ld_x, residual, ld_residual, post_gain, gain, eps, layer_scalar, h, ld_h, d_q,
+                      ld_q, d_scale, x_dtype, h_dtype, q_dtype)
+    check((_lib or load_library()).glp_norm_residual_q8(ctypes.byref(a), stream))
+
+
+def quantize_rows(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dtype: int, d_scale: int, *,
+                  ld_x: int = 0, ld_q: int = 0, stream: int = 0) -> None:
+    """glp_quantize_rows: the 8-bit form (codes and one scale per row) of x [m, h_len]."""
+    check((_lib or load_library()).glp_quantize_rows(d_x, x_dtype, ld_x, m, h_len, d_q, q_dtype, ld_q, d_scale, stream))
+
+
+def linear(m: int, n: int, k: int, dtype: int, d_x: int, d_w: int, d_y: int, out_dtype: int, *, x_scale: int = 0,
+           w_scale: int = 0, w_up: int = 0, w_up_scale: int = 0, bias: int = 0, bias_up: int = 0,
+           activation: int = ACTIVATIONS["none"], residual: int = 0, ldx: int = 0, ldw: int = 0, ld_residual: int = 0,
+           ldy: int = 0, stream: int = 0) -> None:
+    """glp_linear: y = act(x w^T * scales + bias) [* (x w_up^T * scales + bias_up)] + residual.
+    Device pointers as ints (0 = not given), types from ``DTYPES``, ``activation`` from
+    ``ACTIVATIONS``, pitches in elements (0 = packed)."""
+    a = GlpLinearArgs(m, n, k, dtype, d_x, ldx, d_w, w_up, ldw, x_scale, w_scale, w_up_scale, bias, bias_up, residual,
+                      ld_residual, d_y, ldy, out_dtype, activation)
+    check((_lib or load_library()).glp_linear(ctypes.byref(a), stream))
 
 
 def flash_attention(d_qkv: int, d_cu: int, n_seq: int, max_len: int, n_q_heads: int, n_kv_heads: int,

@@ -32,6 +32,7 @@
 #include "gemm.cuh"
 #include "gguf.h"
 #include "glypr_cuda.h"
+#include "operators.h"
 #include "ple.cuh"
 #include "q8gemm.cuh"
 #include "rowops.cuh"
@@ -1956,8 +1957,9 @@ int noalloc_pointers(int dev, __nv_bfloat16** weight, int** status) {
 
 // ================================================================================= C ABI
 namespace glp {
-// for the engine (engine.cpp): set the calling thread's glp_last_error() message
+// for the engine (engine.cpp) and operators.cu: set the calling thread's glp_last_error() message
 void set_last_error(const std::string& msg) { t_err = msg; }
+int kernel_status_word(int dev, int** out) { return device_status_word(dev, out); }
 }  // namespace glp
 
 extern "C" {

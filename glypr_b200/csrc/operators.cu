@@ -1,0 +1,181 @@
+// Host side of the 8-bit row operators and the matrix product with a full epilogue
+// (glp_norm_residual_q8, glp_quantize_rows, glp_linear): argument checks, the choice of kernel,
+// launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <exception>
+#include <string>
+
+#include "glypr_cuda.h"
+#include "linear_any.cuh"
+#include "operators.h"
+#include "rowquant.cuh"
+
+namespace {
+
+using glp::LinearParams;
+using glp::RowQuantParams;
+
+static_assert(GLP_DTYPE_F32 == glp::kF32 && GLP_DTYPE_F16 == glp::kF16 && GLP_DTYPE_BF16 == glp::kBF16 &&
+              GLP_DTYPE_I8 == glp::kI8 && GLP_DTYPE_E4M3 == glp::kE4M3, "dtype codes");
+static_assert(GLP_ACT_NONE == glp::kActNone && GLP_ACT_RELU == glp::kActRelu && GLP_ACT_SILU == glp::kActSilu &&
+              GLP_ACT_GELU_TANH == glp::kActGeluTanh && GLP_ACT_GELU_ERF == glp::kActGeluErf, "activation codes");
+
+int fail(int code, const char* msg) {
+  glp::set_last_error(msg);
+  return code;
+}
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return GLP_OK;
+  glp::set_last_error(std::string("kernel launch: ") + cudaGetErrorString(e));
+  return e == cudaErrorMemoryAllocation ? GLP_ERR_OOM : GLP_ERR_CUDA;
+}
+
+int dtype_size(int dtype) { return dtype == GLP_DTYPE_F32 ? 4 : (dtype == GLP_DTYPE_F16 || dtype == GLP_DTYPE_BF16) ? 2 : 1; }
+bool wide_dtype(int dtype) { return dtype == GLP_DTYPE_F32 || dtype == GLP_DTYPE_F16 || dtype == GLP_DTYPE_BF16; }
+bool code_dtype(int dtype) { return dtype == GLP_DTYPE_I8 || dtype == GLP_DTYPE_E4M3; }
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// a row pitch in elements: 0 = packed; false when shorter than the row
+bool pitch(int64_t* ld, int64_t cols) {
+  if (*ld == 0) *ld = cols;
+  return *ld >= cols;
+}
+
+template <bool NORM>
+int launch_row_quant(const RowQuantParams& p, cudaStream_t st) {
+  const unsigned rows = static_cast<unsigned>(p.M);
+  if (p.H <= 256)
+    glp::row_quant_any_kernel<32, 8, NORM><<<(rows + 3) / 4, 128, 0, st>>>(p);
+  else if (p.H <= 2048)
+    glp::row_quant_any_kernel<128, 16, NORM><<<rows, 128, 0, st>>>(p);
+  else if (p.H <= 8192)
+    glp::row_quant_any_kernel<512, 16, NORM><<<rows, 512, 0, st>>>(p);
+  else
+    glp::row_quant_any_kernel<1024, 32, NORM><<<rows, 1024, 0, st>>>(p);
+  return launched();
+}
+
+int norm_residual_q8(const glp_norm_q8_args* a, cudaStream_t st) {
+  if (!a) return fail(GLP_ERR_INVALID_ARG, "args is NULL");
+  if (a->M < 0 || a->H < 1 || a->H > GLP_QUANT_MAX_H)
+    return fail(GLP_ERR_INVALID_ARG, "norm needs M >= 0 and 1 <= H <= 32768");
+  if (!wide_dtype(a->x_dtype) || !wide_dtype(a->h_dtype)) return fail(GLP_ERR_INVALID_ARG, "x and h must be F32, F16 or BF16");
+  if (!code_dtype(a->q_dtype)) return fail(GLP_ERR_INVALID_ARG, "q must be I8 or E4M3");
+  if (!(a->eps >= 0.0f)) return fail(GLP_ERR_INVALID_ARG, "eps must be >= 0");
+  RowQuantParams p{};
+  p.M = a->M, p.H = a->H;
+  p.x = a->x, p.residual = a->residual, p.post_gain = a->post_gain, p.gain = a->gain;
+  p.h = a->h, p.q = a->q, p.scale = a->scale;
+  p.ld_x = a->ld_x, p.ld_residual = a->ld_residual, p.ld_h = a->ld_h, p.ld_q = a->ld_q;
+  p.eps = a->eps, p.layer_scalar = a->layer_scalar;
+  p.x_dtype = a->x_dtype, p.h_dtype = a->h_dtype, p.q_dtype = a->q_dtype;
+  if (!pitch(&p.ld_x, p.H) || !pitch(&p.ld_residual, p.H) || !pitch(&p.ld_h, p.H) || !pitch(&p.ld_q, p.H))
+    return fail(GLP_ERR_INVALID_ARG, "a row pitch is shorter than H");
+  if (a->M == 0) return GLP_OK;
+  if (!p.x || !p.q || !p.scale) return fail(GLP_ERR_INVALID_ARG, "null pointer");
+  if (p.h && p.h == p.residual && p.ld_h != p.ld_residual)
+    return fail(GLP_ERR_INVALID_ARG, "h in place of residual needs the same row pitch");
+  if (!aligned(p.x, dtype_size(p.x_dtype)) || !aligned(p.residual, dtype_size(p.h_dtype)) ||
+      !aligned(p.h, dtype_size(p.h_dtype)) || !aligned(p.post_gain, 4) || !aligned(p.gain, 4) || !aligned(p.scale, 4))
+    return fail(GLP_ERR_INVALID_ARG, "a pointer is not aligned to its element type");
+  return launch_row_quant<true>(p, st);
+}
+
+int quantize_rows(const void* x, int x_dtype, int64_t ld_x, int M, int H, void* q, int q_dtype, int64_t ld_q,
+                  float* scale, cudaStream_t st) {
+  if (M < 0 || H < 1 || H > GLP_QUANT_MAX_H)
+    return fail(GLP_ERR_INVALID_ARG, "row quantisation needs M >= 0 and 1 <= H <= 32768");
+  if (!wide_dtype(x_dtype)) return fail(GLP_ERR_INVALID_ARG, "x must be F32, F16 or BF16");
+  if (!code_dtype(q_dtype)) return fail(GLP_ERR_INVALID_ARG, "q must be I8 or E4M3");
+  RowQuantParams p{};
+  p.M = M, p.H = H, p.x = x, p.q = q, p.scale = scale, p.ld_x = ld_x, p.ld_q = ld_q;
+  p.x_dtype = x_dtype, p.q_dtype = q_dtype;
+  if (!pitch(&p.ld_x, H) || !pitch(&p.ld_q, H)) return fail(GLP_ERR_INVALID_ARG, "a row pitch is shorter than H");
+  if (M == 0) return GLP_OK;
+  if (!x || !q || !scale) return fail(GLP_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(x, dtype_size(x_dtype)) || !aligned(scale, 4))
+    return fail(GLP_ERR_INVALID_ARG, "a pointer is not aligned to its element type");
+  return launch_row_quant<false>(p, st);
+}
+
+template <int DT>
+int launch_any(const LinearParams& p, cudaStream_t st) {
+  const int64_t tiles = ((p.M + 63ll) / 64) * ((p.N + 63ll) / 64);
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, 1 << 20));
+  if (p.w_up)
+    glp::linear_any_kernel<DT, true><<<grid, 256, 0, st>>>(p);
+  else
+    glp::linear_any_kernel<DT, false><<<grid, 256, 0, st>>>(p);
+  return launched();
+}
+
+int linear(const glp_linear_args* a, cudaStream_t st) {
+  if (!a) return fail(GLP_ERR_INVALID_ARG, "args is NULL");
+  if (a->M < 0 || a->N < 1 || a->K < 1) return fail(GLP_ERR_INVALID_ARG, "linear needs M >= 0, N >= 1, K >= 1");
+  if (a->dtype < GLP_DTYPE_F16 || a->dtype > GLP_DTYPE_E4M3)
+    return fail(GLP_ERR_INVALID_ARG, "operands must be F16, BF16, I8 or E4M3");
+  if (!wide_dtype(a->out_dtype)) return fail(GLP_ERR_INVALID_ARG, "y must be F32, F16 or BF16");
+  if (a->activation < GLP_ACT_NONE || a->activation > GLP_ACT_GELU_ERF)
+    return fail(GLP_ERR_INVALID_ARG, "unknown activation");
+  if (a->dtype == GLP_DTYPE_I8 && a->K > 131071)
+    return fail(GLP_ERR_INVALID_ARG, "int8 operands need K <= 131071 (int32 sums)");
+  if (!a->w_up && (a->w_up_scale || a->bias_up))
+    return fail(GLP_ERR_INVALID_ARG, "w_up_scale and bias_up need w_up");
+  LinearParams p{};
+  p.M = a->M, p.N = a->N, p.K = a->K;
+  p.dtype = a->dtype, p.out_dtype = a->out_dtype, p.activation = a->activation;
+  p.x = a->x, p.w = a->w, p.w_up = a->w_up, p.ld_x = a->ld_x, p.ld_w = a->ld_w;
+  p.x_scale = a->x_scale, p.w_scale = a->w_scale, p.w_up_scale = a->w_up_scale;
+  p.bias = a->bias, p.bias_up = a->bias_up;
+  p.residual = a->residual, p.y = a->y, p.ld_residual = a->ld_residual, p.ld_y = a->ld_y;
+  if (!pitch(&p.ld_x, p.K) || !pitch(&p.ld_w, p.K)) return fail(GLP_ERR_INVALID_ARG, "a row pitch is shorter than K");
+  if (!pitch(&p.ld_residual, p.N) || !pitch(&p.ld_y, p.N)) return fail(GLP_ERR_INVALID_ARG, "a row pitch is shorter than N");
+  if (a->M == 0) return GLP_OK;
+  if (!p.x || !p.w || !p.y) return fail(GLP_ERR_INVALID_ARG, "null pointer");
+  if (p.residual && p.residual == p.y && p.ld_residual != p.ld_y)
+    return fail(GLP_ERR_INVALID_ARG, "y in place of residual needs the same row pitch");
+  const size_t es = dtype_size(p.dtype), os = dtype_size(p.out_dtype);
+  if (!aligned(p.x, es) || !aligned(p.w, es) || !aligned(p.w_up, es) || !aligned(p.y, os) || !aligned(p.residual, os) ||
+      !aligned(p.x_scale, 4) || !aligned(p.w_scale, 4) || !aligned(p.w_up_scale, 4) || !aligned(p.bias, 4) ||
+      !aligned(p.bias_up, 4))
+    return fail(GLP_ERR_INVALID_ARG, "a pointer is not aligned to its element type");
+  switch (p.dtype) {
+    case GLP_DTYPE_F16: return launch_any<glp::kF16>(p, st);
+    case GLP_DTYPE_BF16: return launch_any<glp::kBF16>(p, st);
+    case GLP_DTYPE_I8: return launch_any<glp::kI8>(p, st);
+    default: return launch_any<glp::kE4M3>(p, st);
+  }
+}
+
+// no C++ exception leaves a C entry (an error message is the only allocation)
+template <class F>
+int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception&) {
+    return GLP_ERR_OOM;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int glp_norm_residual_q8(const glp_norm_q8_args* args, void* stream) {
+  return guarded([&] { return norm_residual_q8(args, static_cast<cudaStream_t>(stream)); });
+}
+
+int glp_quantize_rows(const void* x, int x_dtype, int64_t ld_x, int M, int H, void* q, int q_dtype, int64_t ld_q,
+                      float* scale, void* stream) {
+  return guarded([&] { return quantize_rows(x, x_dtype, ld_x, M, H, q, q_dtype, ld_q, scale, static_cast<cudaStream_t>(stream)); });
+}
+
+int glp_linear(const glp_linear_args* args, void* stream) {
+  return guarded([&] { return linear(args, static_cast<cudaStream_t>(stream)); });
+}
+
+}  // extern "C"

@@ -91,6 +91,70 @@ pub type glp_batch_fn = Option<
     ) -> c_int,
 >;
 
+pub const GLP_DTYPE_F32: c_int = 0;
+pub const GLP_DTYPE_F16: c_int = 1;
+pub const GLP_DTYPE_BF16: c_int = 2;
+pub const GLP_DTYPE_I8: c_int = 3;
+pub const GLP_DTYPE_E4M3: c_int = 4;
+pub const GLP_ACT_NONE: c_int = 0;
+pub const GLP_ACT_RELU: c_int = 1;
+pub const GLP_ACT_SILU: c_int = 2;
+pub const GLP_ACT_GELU_TANH: c_int = 3;
+pub const GLP_ACT_GELU_ERF: c_int = 4;
+pub const GLP_QUANT_MAX_H: c_int = 32768;
+
+/// Arguments of `glp_norm_residual_q8` (device pointers; a null one is not given).
+#[allow(non_snake_case)]
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct glp_norm_q8_args {
+    pub M: c_int,
+    pub H: c_int,
+    pub x: *const c_void,
+    pub ld_x: i64,
+    pub residual: *const c_void,
+    pub ld_residual: i64,
+    pub post_gain: *const c_float,
+    pub gain: *const c_float,
+    pub eps: c_float,
+    pub layer_scalar: c_float,
+    pub h: *mut c_void,
+    pub ld_h: i64,
+    pub q: *mut c_void,
+    pub ld_q: i64,
+    pub scale: *mut c_float,
+    pub x_dtype: c_int,
+    pub h_dtype: c_int,
+    pub q_dtype: c_int,
+}
+
+/// Arguments of `glp_linear` (device pointers; a null one is not given).
+#[allow(non_snake_case)]
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct glp_linear_args {
+    pub M: c_int,
+    pub N: c_int,
+    pub K: c_int,
+    pub dtype: c_int,
+    pub x: *const c_void,
+    pub ld_x: i64,
+    pub w: *const c_void,
+    pub w_up: *const c_void,
+    pub ld_w: i64,
+    pub x_scale: *const c_float,
+    pub w_scale: *const c_float,
+    pub w_up_scale: *const c_float,
+    pub bias: *const c_float,
+    pub bias_up: *const c_float,
+    pub residual: *const c_void,
+    pub ld_residual: i64,
+    pub y: *mut c_void,
+    pub ld_y: i64,
+    pub out_dtype: c_int,
+    pub activation: c_int,
+}
+
 extern "C" {
     pub fn glp_open(
         gguf_path: *const c_char,
@@ -315,4 +379,18 @@ extern "C" {
         d_out: *mut c_void,
         stream: *mut c_void,
     ) -> c_int;
+    pub fn glp_norm_residual_q8(args: *const glp_norm_q8_args, stream: *mut c_void) -> c_int;
+    pub fn glp_quantize_rows(
+        x: *const c_void,
+        x_dtype: c_int,
+        ld_x: i64,
+        m: c_int,
+        h: c_int,
+        q: *mut c_void,
+        q_dtype: c_int,
+        ld_q: i64,
+        scale: *mut c_float,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn glp_linear(args: *const glp_linear_args, stream: *mut c_void) -> c_int;
 }

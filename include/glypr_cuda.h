@@ -285,7 +285,7 @@ int glp_q8_0_gemm_noalloc(const void* d_q8_w, int N, int K, const void* d_x_bf16
                           void* stream);
 
 /* Status of the kernel-level entry points above and below (glp_q8_0_gemm, glp_bf16_gemm,
- * glp_flash_attention, glp_q8_0_gemm_noalloc and the fused-epilogue GEMMs) on CUDA device
+ * glp_flash_attention, glp_q8_0_gemm_noalloc, glp_linear and the fused-epilogue GEMMs) on CUDA device
  * `device`: they are stream-ordered and return before their kernels run, so a kernel whose
  * bounded wait expired (its output then undefined) is reported here.  Synchronises the device,
  * then reads and clears the status words of these entry points: *status = the code recorded
@@ -332,6 +332,93 @@ int glp_qkv_norm_rope(const void* d_w_qkv, int n_q_heads, int n_kv_heads, int K,
  * (attention/traits.rs:37-46, AttentionMode::CudaFlash at attention/mod.rs:255-262). */
 int glp_flash_attention(const void* d_qkv, const int32_t* d_cu_seqlens, int n_seq, int max_len, int n_q_heads,
                         int n_kv_heads, int head_dim, int window, void* d_out, void* stream);
+
+/* ---- 8-bit activations and matrix products with a full epilogue (kernel-level; current device) ----
+ *
+ * What a W8A8 layer is made of: rows normalised and written in 8 bits with one scale per row, rows
+ * quantised as they are, and a matrix product over 8-bit or 16-bit operands that adds a bias,
+ * applies an activation or a gate, and adds a residual.  (The reference quantises activations to
+ * int8 inside its CPU matmul, candle's Q8_0 path behind linear.rs:150-172; its linears have no
+ * bias or residual of their own.)  All three are stream-ordered, allocate nothing after the first
+ * call on a device, accept any sizes from 1 up, and take row pitches (ld*, in elements; 0 = the
+ * row's own length). */
+
+/* element types */
+#define GLP_DTYPE_F32 0
+#define GLP_DTYPE_F16 1
+#define GLP_DTYPE_BF16 2
+#define GLP_DTYPE_I8 3   /* int8 codes in [-127, 127] */
+#define GLP_DTYPE_E4M3 4 /* 8-bit floats: 4 exponent and 3 fraction bits, largest 448, no infinities */
+
+/* activations */
+#define GLP_ACT_NONE 0
+#define GLP_ACT_RELU 1
+#define GLP_ACT_SILU 2
+#define GLP_ACT_GELU_TANH 3
+#define GLP_ACT_GELU_ERF 4
+
+#define GLP_QUANT_MAX_H 32768 /* longest row of the two quantising entry points */
+
+/* A row's 8-bit form: scale = max(max|v| / top, 2^-100), code = v / scale rounded to the nearest
+ * code (ties to even); top = 127 (GLP_DTYPE_I8) or 448 (GLP_DTYPE_E4M3), so code * scale is the
+ * value.  A row of zeros has codes 0 and scale 2^-100.  A row that holds a NaN or an infinity has
+ * scale NaN, so that every value it stands for is NaN (codes unspecified). */
+typedef struct glp_norm_q8_args {
+  int M, H;             /* rows and row length, 1 <= H <= GLP_QUANT_MAX_H */
+  const void* x;        /* [M, H] sublayer output, F32 / F16 / BF16 */
+  int64_t ld_x;
+  const void* residual; /* [M, H] of h_dtype, or NULL */
+  int64_t ld_residual;
+  const float* post_gain; /* [H]: x is normalised with it before the addition; NULL: added as it is */
+  const float* gain;      /* [H] gain of the output norm; NULL = ones */
+  float eps;
+  float layer_scalar;   /* h = (residual + x~) * layer_scalar */
+  void* h;              /* [M, H] of h_dtype: the new residual stream, or NULL; may be residual itself */
+  int64_t ld_h;
+  void* q;              /* [M, H] codes of RMSNorm(h) * gain, I8 / E4M3 */
+  int64_t ld_q;
+  float* scale;         /* [M] */
+  int x_dtype, h_dtype, q_dtype;
+} glp_norm_q8_args;
+
+/* The sandwich or pre-norm between two sublayers with its output in 8 bits:
+ *   x~ = x * rms(x) * post_gain (or x),  h = (residual + x~) * layer_scalar,
+ *   (q, scale) = 8-bit form of h * rms(h) * gain,   rms(v) = 1 / sqrt(mean(v^2) + eps),
+ * all in f32; h is rounded once, to h_dtype, and the norm continues from the unrounded value (as
+ * the model path's post_norm_residual does; norm.rs:22-94, layer.rs:20-50). */
+int glp_norm_residual_q8(const glp_norm_q8_args* args, void* stream);
+
+/* q, scale [M] = the 8-bit form of each row of x [M, H] (F32 / F16 / BF16): weights once at load,
+ * and activations that no norm precedes. */
+int glp_quantize_rows(const void* x, int x_dtype, int64_t ld_x, int M, int H, void* q, int q_dtype, int64_t ld_q,
+                      float* scale, void* stream);
+
+typedef struct glp_linear_args {
+  int M, N, K;
+  int dtype;            /* of x, w and w_up: F16, BF16, I8 or E4M3 */
+  const void* x;        /* [M, K] */
+  int64_t ld_x;
+  const void* w;        /* [N, K] */
+  const void* w_up;     /* [N, K]: makes the product gated; NULL = not */
+  int64_t ld_w;         /* of w and w_up */
+  const float* x_scale;    /* [M] scale of each row of x, NULL = ones */
+  const float* w_scale;    /* [N] scale of each row of w, NULL = ones */
+  const float* w_up_scale; /* [N] */
+  const float* bias;       /* [N] or NULL */
+  const float* bias_up;    /* [N] or NULL */
+  const void* residual;    /* [M, N] of out_dtype, or NULL */
+  int64_t ld_residual;
+  void* y;                 /* [M, N] of out_dtype; may be residual itself (with its pitch) */
+  int64_t ld_y;
+  int out_dtype;           /* F32, F16 or BF16 */
+  int activation;          /* GLP_ACT_* */
+} glp_linear_args;
+
+/* y = act(x w^T * x_scale * w_scale + bias) [* (x w_up^T * x_scale * w_up_scale + bias_up)] + residual
+ * with products summed in f32 (I8: exactly, in int32; K <= 131071) and one rounding to out_dtype.
+ * Rows of x, w and w_up that start on 16-byte boundaries (base addresses and pitches) run on the
+ * tensor cores; any other alignment is accepted and slower. */
+int glp_linear(const glp_linear_args* args, void* stream);
 
 #ifdef __cplusplus
 }
