@@ -63,9 +63,7 @@ int fail(int code, const std::string& msg) {
   } while (0)
 
 // ------------------------------------------------------------------------------ TMA maps
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using glp::EncodeTiledFn;
 
 EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
@@ -1960,6 +1958,7 @@ namespace glp {
 // for the engine (engine.cpp) and operators.cu: set the calling thread's glp_last_error() message
 void set_last_error(const std::string& msg) { t_err = msg; }
 int kernel_status_word(int dev, int** out) { return device_status_word(dev, out); }
+EncodeTiledFn tensor_map_encoder() { return encode_fn(); }
 }  // namespace glp
 
 extern "C" {

@@ -2,46 +2,9 @@
 // 64 x 64 output tiles, 256 threads of 4 x 4 outputs, 16 columns of K at a time through shared
 // memory, one element per load.  Products are f32 FMAs (int8: exact int32 sums).
 #pragma once
-#include "common.cuh"
-#include "rowquant.cuh"
+#include "linear.cuh"
 
 namespace glp {
-
-enum Activation : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGeluTanh = 3, kActGeluErf = 4 };
-
-struct LinearParams {
-  int M, N, K;
-  int dtype, out_dtype, activation;
-  const void* x;
-  const void* w;
-  const void* w_up;
-  int64_t ld_x, ld_w;
-  const float* x_scale;
-  const float* w_scale;
-  const float* w_up_scale;
-  const float* bias;
-  const float* bias_up;
-  const void* residual;
-  void* y;
-  int64_t ld_residual, ld_y;
-  int* status;
-};
-
-// act(v).  SiLU is v / (1 + e^-v) and tanh-GELU v / (1 + e^-2z), z = sqrt(2/pi) (v + 0.044715 v^3):
-// 0.5 (1 + tanh z) without its cancellation.  For v so negative that the exponential overflows the
-// quotient is -0, the limit.
-__device__ __forceinline__ float activate(float v, int kind) {
-  switch (kind) {
-    case kActRelu: return v < 0.0f ? 0.0f : v;  // a NaN stays
-    case kActSilu: return __fdividef(v, 1.0f + __expf(-v));
-    case kActGeluTanh: {
-      const float z2 = -1.5957691216f * fmaf(0.044715f * v, v * v, v);
-      return __fdividef(v, 1.0f + __expf(z2));
-    }
-    case kActGeluErf: return 0.5f * v * erfcf(-0.70710678f * v);
-    default: return v;
-  }
-}
 
 __device__ __forceinline__ float e4m3_to_f32(uint8_t c) {
   uint32_t h2;

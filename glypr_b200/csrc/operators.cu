@@ -4,11 +4,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <exception>
 #include <string>
 
 #include "glypr_cuda.h"
 #include "linear_any.cuh"
+#include "linear_tc.cuh"
 #include "operators.h"
 #include "rowquant.cuh"
 
@@ -113,6 +115,122 @@ int launch_any(const LinearParams& p, cudaStream_t st) {
   return launched();
 }
 
+// ------------------------------------------------------------------------------ tensor-core product
+// a row-major [rows, cols] matrix in boxes of box_rows rows x 128 bytes, 128-byte swizzle, zeros
+// outside.  Encoded on every call: a map is a function of these arguments alone.
+int make_map(CUtensorMap* m, const void* base, int dtype, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  const glp::EncodeTiledFn fn = glp::tensor_map_encoder();
+  if (!fn) return fail(GLP_ERR_CUDA, "cuTensorMapEncodeTiled unavailable (driver too old?)");
+  const int size = dtype_size(dtype);
+  const CUtensorMapDataType type = size == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * size)};
+  const cuuint32_t box[2] = {128u / size, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return GLP_OK;
+  glp::set_last_error("cuTensorMapEncodeTiled failed: " + std::to_string(r));
+  return GLP_ERR_CUDA;
+}
+
+struct DeviceInfo {
+  int dev, sms;
+  int* status;
+};
+
+int device_info(DeviceInfo* d) {
+  static std::atomic<int> sms[64];
+  if (cudaGetDevice(&d->dev) != cudaSuccess || d->dev < 0 || d->dev >= 64)
+    return fail(GLP_ERR_CUDA, "no usable CUDA device");
+  d->sms = sms[d->dev].load(std::memory_order_relaxed);
+  if (!d->sms) {
+    if (cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, d->dev) != cudaSuccess || d->sms < 1)
+      return fail(GLP_ERR_CUDA, "cannot read the device's SM count");
+    sms[d->dev].store(d->sms, std::memory_order_relaxed);
+  }
+  return glp::kernel_status_word(d->dev, &d->status);
+}
+
+// Instruction descriptor: f32 (int8: s32) accumulator, both operands K-major, m x n.
+uint32_t mma_idesc(int dtype, int m, int n) {
+  const uint32_t acc = dtype == GLP_DTYPE_I8 ? 2u : 1u;                                   // s32 | f32
+  const uint32_t ab = (dtype == GLP_DTYPE_BF16 || dtype == GLP_DTYPE_I8) ? 1u : 0u;  // bf16, s8 | f16, e4m3
+  return acc << 4 | ab << 7 | ab << 10 | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
+}
+
+template <int KIND, int CG, int BN, bool GATED>
+int launch_tc(glp::LinearTcParams p, const DeviceInfo& d, cudaStream_t st) {
+  using Cfg = glp::LinearTcCfg<CG, BN, GATED>;
+  const auto kernel = glp::linear_tc_kernel<KIND, CG, BN, GATED>;
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+  const uint64_t bit = 1ull << d.dev;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::SMEM));
+    if (e != cudaSuccess) return fail(GLP_ERR_CUDA, cudaGetErrorString(e));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const LinearParams& a = p.a;
+  p.m_tiles = (a.M + 128 * CG - 1) / (128 * CG);
+  p.n_tiles = (a.N + Cfg::OUT_N - 1) / Cfg::OUT_N;
+  p.k_step = 128 / dtype_size(a.dtype);
+  p.k_blocks = (a.K + p.k_step - 1) / p.k_step;
+  p.idesc = mma_idesc(a.dtype, 128 * CG, BN);
+  const size_t os = dtype_size(a.out_dtype);
+  p.tma_out = aligned(a.y, 16) && a.ld_y * os % 16 == 0 &&
+              (!a.residual || (aligned(a.residual, 16) && a.ld_residual * os % 16 == 0));
+  // rows of w (and of w_up) that one load brings: a gated single CTA takes half of each
+  const int w_rows = CG == 2 ? BN / 2 : Cfg::OUT_N;
+  CUtensorMap mx, mw, mu, mr, my;
+  if (int rc = make_map(&mx, a.x, a.dtype, a.M, a.K, a.ld_x, 128)) return rc;
+  if (int rc = make_map(&mw, a.w, a.dtype, a.N, a.K, a.ld_w, w_rows)) return rc;
+  mu = mr = my = mw;
+  if (GATED)
+    if (int rc = make_map(&mu, a.w_up, a.dtype, a.N, a.K, a.ld_w, w_rows)) return rc;
+  if (p.tma_out) {
+    if (int rc = make_map(&my, a.y, a.out_dtype, a.M, a.N, a.ld_y, 32)) return rc;
+    if (a.residual)
+      if (int rc = make_map(&mr, a.residual, a.out_dtype, a.M, a.N, a.ld_residual, 32)) return rc;
+  }
+  const int units = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.m_tiles) * p.n_tiles, d.sms / CG));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mx, mw, mu, mr, my, p);
+  if (e == cudaSuccess) return GLP_OK;
+  glp::set_last_error(std::string("kernel launch: ") + cudaGetErrorString(e));
+  return GLP_ERR_CUDA;
+}
+
+template <int KIND>
+int launch_tc_kind(const LinearParams& a, const DeviceInfo& d, cudaStream_t st) {
+  glp::LinearTcParams p{};
+  p.a = a;
+  p.a.status = d.status;
+  const bool gated = a.w_up != nullptr;
+  const int64_t rows128 = (a.M + 127) / 128, pairs = ((a.M + 255ll) / 256) * ((a.N + (gated ? 127ll : 255ll)) / (gated ? 128 : 256));
+  if (pairs >= d.sms / 2) return gated ? launch_tc<KIND, 2, 256, true>(p, d, st) : launch_tc<KIND, 2, 256, false>(p, d, st);
+  if (gated) return launch_tc<KIND, 1, 128, true>(p, d, st);
+  if (rows128 * ((a.N + 127ll) / 128) >= d.sms / 2) return launch_tc<KIND, 1, 128, false>(p, d, st);
+  return launch_tc<KIND, 1, 64, false>(p, d, st);
+}
+
+bool tc_operands(const LinearParams& p) {
+  const size_t es = dtype_size(p.dtype);
+  return aligned(p.x, 16) && aligned(p.w, 16) && aligned(p.w_up, 16) && p.ld_x * es % 16 == 0 && p.ld_w * es % 16 == 0;
+}
+
 int linear(const glp_linear_args* a, cudaStream_t st) {
   if (!a) return fail(GLP_ERR_INVALID_ARG, "args is NULL");
   if (a->M < 0 || a->N < 1 || a->K < 1) return fail(GLP_ERR_INVALID_ARG, "linear needs M >= 0, N >= 1, K >= 1");
@@ -143,6 +261,13 @@ int linear(const glp_linear_args* a, cudaStream_t st) {
       !aligned(p.x_scale, 4) || !aligned(p.w_scale, 4) || !aligned(p.w_up_scale, 4) || !aligned(p.bias, 4) ||
       !aligned(p.bias_up, 4))
     return fail(GLP_ERR_INVALID_ARG, "a pointer is not aligned to its element type");
+  if (tc_operands(p)) {
+    DeviceInfo d;
+    if (int rc = device_info(&d)) return rc;
+    if (p.dtype == GLP_DTYPE_I8) return launch_tc_kind<glp::kMmaI8>(p, d, st);
+    if (p.dtype == GLP_DTYPE_E4M3) return launch_tc_kind<glp::kMmaE4M3>(p, d, st);
+    return launch_tc_kind<glp::kMmaF16>(p, d, st);
+  }
   switch (p.dtype) {
     case GLP_DTYPE_F16: return launch_any<glp::kF16>(p, st);
     case GLP_DTYPE_BF16: return launch_any<glp::kBF16>(p, st);
