@@ -47,8 +47,50 @@ bool pitch(int64_t* ld, int64_t cols) {
   return *ld >= cols;
 }
 
+template <int G, int NC, bool NORM>
+int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
+  constexpr int ROWS = G == 32 ? 8 : 1;
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.M) + ROWS - 1) / ROWS), block = G == 32 ? 256 : G;
+  const bool x4 = p.x_dtype == GLP_DTYPE_F32, h4 = NORM && p.h_dtype == GLP_DTYPE_F32;
+  if (!x4 && !h4) glp::row_quant_kernel<G, NC, 2, 2, NORM><<<grid, block, 0, st>>>(p, gains16);
+  if (x4 && !h4) glp::row_quant_kernel<G, NC, 4, 2, NORM><<<grid, block, 0, st>>>(p, gains16);
+  if constexpr (NORM) {
+    if (!x4 && h4) glp::row_quant_kernel<G, NC, 2, 4, NORM><<<grid, block, 0, st>>>(p, gains16);
+    if (x4 && h4) glp::row_quant_kernel<G, NC, 4, 4, NORM><<<grid, block, 0, st>>>(p, gains16);
+  }
+  return launched();
+}
+
+// Whether every row's x, residual, h and q stand at the same place in their chunks of 8 elements.
+bool same_chunks(const RowQuantParams& p) {
+  const auto place = [](const void* a, int size) { return reinterpret_cast<uintptr_t>(a) / size % 8; };
+  const int xs = dtype_size(p.x_dtype), hs = dtype_size(p.h_dtype);
+  const uintptr_t x = place(p.x, xs);
+  return place(p.q, 1) == x && (p.ld_q - p.ld_x) % 8 == 0 &&
+         (!p.residual || (place(p.residual, hs) == x && (p.ld_residual - p.ld_x) % 8 == 0)) &&
+         (!p.h || (place(p.h, hs) == x && (p.ld_h - p.ld_x) % 8 == 0));
+}
+
 template <bool NORM>
 int launch_row_quant(const RowQuantParams& p, cudaStream_t st) {
+  if (same_chunks(p)) {
+    const bool gains16 = aligned(p.gain, 16) && aligned(p.post_gain, 16);
+    // a row that starts inside a chunk touches one more
+    const int dx = dtype_size(p.x_dtype);
+    const bool flush = reinterpret_cast<uintptr_t>(p.x) / dx % 8 == 0 && p.ld_x % 8 == 0;
+    const int chunks = (p.H + (flush ? 7 : 14)) / 8;
+    if (chunks <= 32) return launch_chunks<32, 1, NORM>(p, gains16, st);
+    if (chunks <= 64) return launch_chunks<32, 2, NORM>(p, gains16, st);
+    if (chunks <= 96) return launch_chunks<32, 3, NORM>(p, gains16, st);
+    if (chunks <= 128) return launch_chunks<32, 4, NORM>(p, gains16, st);
+    if (chunks <= 256) return launch_chunks<128, 2, NORM>(p, gains16, st);
+    if (chunks <= 384) return launch_chunks<128, 3, NORM>(p, gains16, st);
+    if (chunks <= 512) return launch_chunks<128, 4, NORM>(p, gains16, st);
+    if (chunks <= 1024) return launch_chunks<512, 2, NORM>(p, gains16, st);
+    if (chunks <= 1536) return launch_chunks<512, 3, NORM>(p, gains16, st);
+    if (chunks <= 2048) return launch_chunks<512, 4, NORM>(p, gains16, st);
+    if (chunks <= 4096) return launch_chunks<1024, 4, NORM>(p, gains16, st);
+  }
   const unsigned rows = static_cast<unsigned>(p.M);
   if (p.H <= 256)
     glp::row_quant_any_kernel<32, 8, NORM><<<(rows + 3) / 4, 128, 0, st>>>(p);

@@ -159,4 +159,237 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
   }
 }
 
+// ---------------------------------------------------------------------------- 8 elements at a time
+// The same rows in aligned chunks of 8 elements (one 16-byte load of a 16-bit row, two of an f32 row,
+// one 8-byte store of codes).  Rows need not start on a chunk boundary -- a packed odd width has no two
+// rows alike -- as long as x, residual, h and q all stand at the same place in their chunks: chunk i of
+// a row is elements [8 i - off, 8 i - off + 8), and only the two at the row's ends go by element.
+template <int B>
+struct Chunk {  // 8 raw elements of B bytes
+  uint4 v[B / 2];
+};
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no line in L1
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// elements [e, e + 8) of the row at `row`, zeros outside [0, H)
+template <int B>
+__device__ __forceinline__ Chunk<B> load_chunk(const uint8_t* row, int e, int H) {
+  Chunk<B> c;
+  if (e >= 0 && e + 8 <= H) {
+#pragma unroll
+    for (int i = 0; i < B / 2; ++i) c.v[i] = ld_stream(row + static_cast<int64_t>(e) * B + 16 * i);
+  } else {
+    uint32_t w[2 * B];
+#pragma unroll
+    for (int i = 0; i < 2 * B; ++i) w[i] = 0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int n = e + j;
+      if (n >= 0 && n < H) {
+        if constexpr (B == 4)
+          w[j] = *reinterpret_cast<const uint32_t*>(row + static_cast<int64_t>(n) * 4);
+        else
+          w[j / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + static_cast<int64_t>(n) * 2)) << (16 * (j & 1));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < B / 2; ++i) c.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+  return c;
+}
+
+template <int B>
+__device__ __forceinline__ void chunk_f32(const Chunk<B>& c, int dtype, float (&v)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&c);
+  if constexpr (B == 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+  } else if (dtype == kBF16) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(w[j] << 16);
+      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+
+template <int B>
+__device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, int dtype, const float (&v)[8]) {
+  if (e >= 0 && e + 8 <= H) {
+    uint8_t* at = row + static_cast<int64_t>(e) * B;
+    if constexpr (B == 4) {
+      *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<float4*>(at + 16) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = dtype == kBF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : *reinterpret_cast<const uint32_t*>(&h);
+      }
+      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (e + j >= 0 && e + j < H) store_from_f32(row, e + j, dtype, v[j]);
+  }
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dtype, const float (&v)[8], float k) {
+  uint32_t w[2];
+  if (q_dtype == kI8) {
+    // v * k + 1.5 * 2^23 rounds once to the nearest integer, ties to even, and leaves it in the low byte
+    uint32_t b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(fmaf(v[j], k, 12582912.0f));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      w[i] = code_e4m3x2(v[4 * i] * k, v[4 * i + 1] * k) |
+             static_cast<uint32_t>(code_e4m3x2(v[4 * i + 2] * k, v[4 * i + 3] * k)) << 16;
+  }
+  if (e >= 0 && e + 8 <= H) {
+    *reinterpret_cast<uint2*>(row + e) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (e + j >= 0 && e + j < H) row[e + j] = static_cast<uint8_t>(w[j / 4] >> (8 * (j & 3)));
+  }
+}
+
+// gain[e .. e + 8), ones where there is none (outside [0, H) the value does not matter).  e is a
+// multiple of 8 less the row's off: the aligned words around it are loaded and shifted by off & 3,
+// which is the same for the whole row.
+__device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, int H, float (&v)[8]) {
+  if (!gain) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 1.0f;
+    return;
+  }
+  const int s = e & 3;
+  if (aligned16 && e - s >= 0 && e - s + (s ? 12 : 8) <= H) {
+    float w[12];
+    const float4* at = reinterpret_cast<const float4*>(gain + (e - s));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const float4 f = i < 2 || s ? __ldg(at + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      w[4 * i] = f.x, w[4 * i + 1] = f.y, w[4 * i + 2] = f.z, w[4 * i + 3] = f.w;
+    }
+    // a shift by s in two steps, so that every index is known at compile time
+#pragma unroll
+    for (int j = 0; j < 10; ++j) w[j] = s & 2 ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = s & 1 ? w[j + 1] : w[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = e + j >= 0 && e + j < H ? __ldg(gain + e + j) : 0.0f;
+  }
+}
+
+// G threads per row, NC chunks per thread: H + 7 <= 8 G NC.  XB, HB: bytes per element of x and of
+// residual / h.  gains16: both gains start on 16-byte boundaries.
+template <int G, int NC, int XB, int HB, bool NORM>
+__global__ void __launch_bounds__(G < 256 ? (G == 32 ? 256 : G) : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
+  constexpr int ROWS = G == 32 ? 8 : 1;
+  const int t = threadIdx.x % G;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G;
+  if (row >= p.M) return;  // whole warps or the whole block
+  const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * XB;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(xr) / XB & 7);
+  Chunk<XB> xc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XB>(xr, (c * G + t) * 8 - off, p.H);
+  uint8_t* qr = static_cast<uint8_t*>(p.q) + row * p.ld_q;
+  float v[NC][8];
+  float none = 0.0f;
+  if constexpr (NORM) {
+    const uint8_t* rr = static_cast<const uint8_t*>(p.residual) + row * p.ld_residual * HB;
+    uint8_t* hr = static_cast<uint8_t*>(p.h) + row * p.ld_h * HB;
+    Chunk<HB> rc[NC];
+    if (p.residual) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HB>(rr, (c * G + t) * 8 - off, p.H);
+    }
+    float inv = 1.0f;
+    if (p.post_gain) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float x[8];
+        chunk_f32<XB>(xc[c], p.x_dtype, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+      }
+      row_reduce<G>(ss, none);
+      inv = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+    }
+    float ss = 0.0f, amax = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int e = (c * G + t) * 8 - off;
+      float g[8];
+      chunk_f32<XB>(xc[c], p.x_dtype, v[c]);
+      if (p.post_gain) {
+        load_gain(p.post_gain, gains16, e, p.H, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] = v[c][j] * inv * g[j];
+      }
+      if (p.residual) {
+        float r[8];
+        chunk_f32<HB>(rc[c], p.h_dtype, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] += r[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[c][j] *= p.layer_scalar;
+        ss = fmaf(v[c][j], v[c][j], ss);
+      }
+      if (p.h) store_chunk<HB>(hr, e, p.H, p.h_dtype, v[c]);
+      load_gain(p.gain, gains16, e, p.H, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[c][j] *= g[j];
+        amax = max_nan(amax, fabsf(v[c][j]));
+      }
+    }
+    row_reduce<G>(ss, amax);
+    const float inv_h = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+    const float s = scale_of(amax * inv_h, p.q_dtype);
+    const float k = inv_h / s;
+    if (t == 0) p.scale[row] = s;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], k);
+  } else {
+    float amax = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      chunk_f32<XB>(xc[c], p.x_dtype, v[c]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[c][j]));
+    }
+    row_reduce<G>(none, amax);
+    const float s = scale_of(amax, p.q_dtype);
+    const float k = 1.0f / s;
+    if (t == 0) p.scale[row] = s;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], k);
+  }
+}
+
 }  // namespace glp
