@@ -7,6 +7,7 @@
 #include <atomic>
 #include <exception>
 #include <string>
+#include <type_traits>
 
 #include "glypr_cuda.h"
 #include "linear_any.cuh"
@@ -51,12 +52,20 @@ template <int G, int NC, bool NORM>
 int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
   constexpr int ROWS = G == 32 ? 8 : 1;
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.M) + ROWS - 1) / ROWS), block = G == 32 ? 256 : G;
-  const bool x4 = p.x_dtype == GLP_DTYPE_F32, h4 = NORM && p.h_dtype == GLP_DTYPE_F32;
-  if (!x4 && !h4) glp::row_quant_kernel<G, NC, 2, 2, NORM><<<grid, block, 0, st>>>(p, gains16);
-  if (x4 && !h4) glp::row_quant_kernel<G, NC, 4, 2, NORM><<<grid, block, 0, st>>>(p, gains16);
   if constexpr (NORM) {
-    if (!x4 && h4) glp::row_quant_kernel<G, NC, 2, 4, NORM><<<grid, block, 0, st>>>(p, gains16);
-    if (x4 && h4) glp::row_quant_kernel<G, NC, 4, 4, NORM><<<grid, block, 0, st>>>(p, gains16);
+    const auto with_h = [&](auto xt) {
+      constexpr int XT = decltype(xt)::value;
+      if (p.h_dtype == GLP_DTYPE_F32) glp::row_quant_kernel<G, NC, XT, glp::kF32, true><<<grid, block, 0, st>>>(p, gains16);
+      if (p.h_dtype == GLP_DTYPE_F16) glp::row_quant_kernel<G, NC, XT, glp::kF16, true><<<grid, block, 0, st>>>(p, gains16);
+      if (p.h_dtype == GLP_DTYPE_BF16) glp::row_quant_kernel<G, NC, XT, glp::kBF16, true><<<grid, block, 0, st>>>(p, gains16);
+    };
+    if (p.x_dtype == GLP_DTYPE_F32) with_h(std::integral_constant<int, glp::kF32>{});
+    if (p.x_dtype == GLP_DTYPE_F16) with_h(std::integral_constant<int, glp::kF16>{});
+    if (p.x_dtype == GLP_DTYPE_BF16) with_h(std::integral_constant<int, glp::kBF16>{});
+  } else {
+    if (p.x_dtype == GLP_DTYPE_F32) glp::row_quant_kernel<G, NC, glp::kF32, glp::kF32, false><<<grid, block, 0, st>>>(p, false);
+    if (p.x_dtype == GLP_DTYPE_F16) glp::row_quant_kernel<G, NC, glp::kF16, glp::kF16, false><<<grid, block, 0, st>>>(p, false);
+    if (p.x_dtype == GLP_DTYPE_BF16) glp::row_quant_kernel<G, NC, glp::kBF16, glp::kBF16, false><<<grid, block, 0, st>>>(p, false);
   }
   return launched();
 }
@@ -83,11 +92,10 @@ int launch_row_quant(const RowQuantParams& p, cudaStream_t st) {
     if (chunks <= 64) return launch_chunks<32, 2, NORM>(p, gains16, st);
     if (chunks <= 96) return launch_chunks<32, 3, NORM>(p, gains16, st);
     if (chunks <= 128) return launch_chunks<32, 4, NORM>(p, gains16, st);
+    if (chunks <= 160) return launch_chunks<32, 5, NORM>(p, gains16, st);
     if (chunks <= 256) return launch_chunks<128, 2, NORM>(p, gains16, st);
-    if (chunks <= 384) return launch_chunks<128, 3, NORM>(p, gains16, st);
     if (chunks <= 512) return launch_chunks<128, 4, NORM>(p, gains16, st);
     if (chunks <= 1024) return launch_chunks<512, 2, NORM>(p, gains16, st);
-    if (chunks <= 1536) return launch_chunks<512, 3, NORM>(p, gains16, st);
     if (chunks <= 2048) return launch_chunks<512, 4, NORM>(p, gains16, st);
     if (chunks <= 4096) return launch_chunks<1024, 4, NORM>(p, gains16, st);
   }

@@ -164,9 +164,12 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
 // one 8-byte store of codes).  Rows need not start on a chunk boundary -- a packed odd width has no two
 // rows alike -- as long as x, residual, h and q all stand at the same place in their chunks: chunk i of
 // a row is elements [8 i - off, 8 i - off + 8), and only the two at the row's ends go by element.
-template <int B>
-struct Chunk {  // 8 raw elements of B bytes
-  uint4 v[B / 2];
+template <int DT>
+constexpr int kBytes = DT == kF32 ? 4 : 2;
+
+template <int DT>
+struct Chunk {  // 8 raw elements
+  uint4 v[kBytes<DT> / 2];
 };
 
 __device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no line in L1
@@ -176,9 +179,10 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no li
 }
 
 // elements [e, e + 8) of the row at `row`, zeros outside [0, H)
-template <int B>
-__device__ __forceinline__ Chunk<B> load_chunk(const uint8_t* row, int e, int H) {
-  Chunk<B> c;
+template <int DT>
+__device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, int H) {
+  constexpr int B = kBytes<DT>;
+  Chunk<DT> c;
   if (e >= 0 && e + 8 <= H) {
 #pragma unroll
     for (int i = 0; i < B / 2; ++i) c.v[i] = ld_stream(row + static_cast<int64_t>(e) * B + 16 * i);
@@ -202,30 +206,29 @@ __device__ __forceinline__ Chunk<B> load_chunk(const uint8_t* row, int e, int H)
   return c;
 }
 
-template <int B>
-__device__ __forceinline__ void chunk_f32(const Chunk<B>& c, int dtype, float (&v)[8]) {
+// as four packed f32 pairs
+template <int DT>
+__device__ __forceinline__ void chunk_f32(const Chunk<DT>& c, uint64_t (&v)[4]) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&c);
-  if constexpr (B == 4) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
-  } else if (dtype == kBF16) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = __uint_as_float(w[j] << 16);
-      v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == kF32) {
+      v[j] = f2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    } else if constexpr (DT == kBF16) {
+      v[j] = f2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+    } else {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
+      v[j] = f2(f.x, f.y);
     }
   }
 }
 
-template <int B>
-__device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, int dtype, const float (&v)[8]) {
+template <int DT>
+__device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, const uint64_t (&p)[4]) {
+  constexpr int B = kBytes<DT>;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f2_split(p[j], v[2 * j], v[2 * j + 1]);
   if (e >= 0 && e + 8 <= H) {
     uint8_t* at = row + static_cast<int64_t>(e) * B;
     if constexpr (B == 4) {
@@ -235,33 +238,44 @@ __device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, int dtyp
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = dtype == kBF16 ? pack_bf16(v[2 * j], v[2 * j + 1]) : *reinterpret_cast<const uint32_t*>(&h);
+        if constexpr (DT == kBF16) {
+          w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        } else {
+          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
       }
       *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (e + j >= 0 && e + j < H) store_from_f32(row, e + j, dtype, v[j]);
+      if (e + j >= 0 && e + j < H) store_from_f32(row, e + j, DT, v[j]);
   }
 }
 
-__device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dtype, const float (&v)[8], float k) {
+__device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dtype, const uint64_t (&p)[4], uint64_t k) {
   uint32_t w[2];
   if (q_dtype == kI8) {
     // v * k + 1.5 * 2^23 rounds once to the nearest integer, ties to even, and leaves it in the low byte
-    uint32_t b[8];
+    float b[8];
+    const uint64_t magic = f2(12582912.0f, 12582912.0f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(fmaf(v[j], k, 12582912.0f));
+    for (int j = 0; j < 4; ++j) f2_split(f2_fma(p[j], k, magic), b[2 * j], b[2 * j + 1]);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+      w[i] = __byte_perm(__byte_perm(__float_as_uint(b[4 * i]), __float_as_uint(b[4 * i + 1]), 0x0040),
+                         __byte_perm(__float_as_uint(b[4 * i + 2]), __float_as_uint(b[4 * i + 3]), 0x0040), 0x5410);
   } else {
+    uint32_t h[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      w[i] = code_e4m3x2(v[4 * i] * k, v[4 * i + 1] * k) |
-             static_cast<uint32_t>(code_e4m3x2(v[4 * i + 2] * k, v[4 * i + 3] * k)) << 16;
+    for (int j = 0; j < 4; ++j) {
+      float lo, hi;
+      f2_split(f2_mul(p[j], k), lo, hi);
+      h[j] = code_e4m3x2(lo, hi);
+    }
+    w[0] = __byte_perm(h[0], h[1], 0x5410);
+    w[1] = __byte_perm(h[2], h[3], 0x5410);
   }
   if (e >= 0 && e + 8 <= H) {
     *reinterpret_cast<uint2*>(row + e) = make_uint2(w[0], w[1]);
@@ -272,22 +286,33 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dt
   }
 }
 
-// gain[e .. e + 8), ones where there is none (outside [0, H) the value does not matter).  e is a
-// multiple of 8 less the row's off: the aligned words around it are loaded and shifted by off & 3,
-// which is the same for the whole row.
-__device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, int H, float (&v)[8]) {
-  if (!gain) {
+// largest magnitude of m and 8 values, keeping a NaN
+__device__ __forceinline__ float max8(float m, const uint64_t (&p)[4]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 1.0f;
+  for (int j = 0; j < 4; ++j) {
+    float lo, hi;
+    f2_split(p[j], lo, hi);
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(lo), "f"(hi));
+  }
+  return m;
+}
+
+// gain[e .. e + 8) (outside [0, H) any finite value).  e is a multiple of 8 less the row's off: for an
+// unaligned row the aligned words around it are loaded and shifted by off & 3, the same for the whole row.
+__device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, int H, uint64_t (&p)[4]) {
+  const int s = e & 3;
+  if (aligned16 && s == 0 && e >= 0 && e + 8 <= H) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(gain + e)), b = __ldg(reinterpret_cast<const float4*>(gain + e) + 1);
+    p[0] = f2(a.x, a.y), p[1] = f2(a.z, a.w), p[2] = f2(b.x, b.y), p[3] = f2(b.z, b.w);
     return;
   }
-  const int s = e & 3;
-  if (aligned16 && e - s >= 0 && e - s + (s ? 12 : 8) <= H) {
+  float v[8];
+  if (aligned16 && e - s >= 0 && e - s + 12 <= H) {
     float w[12];
     const float4* at = reinterpret_cast<const float4*>(gain + (e - s));
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      const float4 f = i < 2 || s ? __ldg(at + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 f = __ldg(at + i);
       w[4 * i] = f.x, w[4 * i + 1] = f.y, w[4 * i + 2] = f.z, w[4 * i + 3] = f.w;
     }
     // a shift by s in two steps, so that every index is known at compile time
@@ -299,96 +324,106 @@ __device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = e + j >= 0 && e + j < H ? __ldg(gain + e + j) : 0.0f;
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p[j] = f2(v[2 * j], v[2 * j + 1]);
 }
 
-// G threads per row, NC chunks per thread: H + 7 <= 8 G NC.  XB, HB: bytes per element of x and of
-// residual / h.  gains16: both gains start on 16-byte boundaries.
-template <int G, int NC, int XB, int HB, bool NORM>
-__global__ void __launch_bounds__(G < 256 ? (G == 32 ? 256 : G) : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
+__device__ __forceinline__ float f2_hsum(uint64_t v) {
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return lo + hi;
+}
+
+// G threads per row, NC chunks per thread: the row touches at most G NC chunks.  XT, HT: types of x and
+// of residual / h.  gains16: both gains start on 16-byte boundaries.
+template <int G, int NC, int XT, int HT, bool NORM>
+__global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
   constexpr int ROWS = G == 32 ? 8 : 1;
   const int t = threadIdx.x % G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G;
   if (row >= p.M) return;  // whole warps or the whole block
-  const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * XB;
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(xr) / XB & 7);
-  Chunk<XB> xc[NC];
+  const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * kBytes<XT>;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
+  Chunk<XT> xc[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XB>(xr, (c * G + t) * 8 - off, p.H);
+  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, (c * G + t) * 8 - off, p.H);
   uint8_t* qr = static_cast<uint8_t*>(p.q) + row * p.ld_q;
-  float v[NC][8];
-  float none = 0.0f;
+  uint64_t v[NC][4];
+  float none = 0.0f, amax = 0.0f;
   if constexpr (NORM) {
-    const uint8_t* rr = static_cast<const uint8_t*>(p.residual) + row * p.ld_residual * HB;
-    uint8_t* hr = static_cast<uint8_t*>(p.h) + row * p.ld_h * HB;
-    Chunk<HB> rc[NC];
+    const uint8_t* rr = static_cast<const uint8_t*>(p.residual) + row * p.ld_residual * kBytes<HT>;
+    uint8_t* hr = static_cast<uint8_t*>(p.h) + row * p.ld_h * kBytes<HT>;
+    Chunk<HT> rc[NC];
     if (p.residual) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HB>(rr, (c * G + t) * 8 - off, p.H);
+      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT>(rr, (c * G + t) * 8 - off, p.H);
     }
-    float inv = 1.0f;
+    uint64_t inv2 = f2(1.0f, 1.0f);
     if (p.post_gain) {
-      float ss = 0.0f;
+      uint64_t ss2 = f2(0.0f, 0.0f);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        float x[8];
-        chunk_f32<XB>(xc[c], p.x_dtype, x);
+        uint64_t x[4];
+        chunk_f32<XT>(xc[c], x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+        for (int j = 0; j < 4; ++j) ss2 = f2_fma(x[j], x[j], ss2);
       }
+      float ss = f2_hsum(ss2);
       row_reduce<G>(ss, none);
-      inv = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+      const float inv = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+      inv2 = f2(inv, inv);
     }
-    float ss = 0.0f, amax = 0.0f;
+    const uint64_t scalar2 = f2(p.layer_scalar, p.layer_scalar);
+    uint64_t ss2 = f2(0.0f, 0.0f);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int e = (c * G + t) * 8 - off;
-      float g[8];
-      chunk_f32<XB>(xc[c], p.x_dtype, v[c]);
+      uint64_t g[4];
+      chunk_f32<XT>(xc[c], v[c]);
       if (p.post_gain) {
         load_gain(p.post_gain, gains16, e, p.H, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[c][j] = v[c][j] * inv * g[j];
+        for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(f2_mul(v[c][j], inv2), g[j]);
       }
       if (p.residual) {
-        float r[8];
-        chunk_f32<HB>(rc[c], p.h_dtype, r);
+        uint64_t r[4];
+        chunk_f32<HT>(rc[c], r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[c][j] += r[j];
+        for (int j = 0; j < 4; ++j) v[c][j] = f2_add(v[c][j], r[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[c][j] *= p.layer_scalar;
-        ss = fmaf(v[c][j], v[c][j], ss);
+      for (int j = 0; j < 4; ++j) {
+        v[c][j] = f2_mul(v[c][j], scalar2);
+        ss2 = f2_fma(v[c][j], v[c][j], ss2);
       }
-      if (p.h) store_chunk<HB>(hr, e, p.H, p.h_dtype, v[c]);
-      load_gain(p.gain, gains16, e, p.H, g);
+      if (p.h) store_chunk<HT>(hr, e, p.H, v[c]);
+      if (p.gain) {
+        load_gain(p.gain, gains16, e, p.H, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[c][j] *= g[j];
-        amax = max_nan(amax, fabsf(v[c][j]));
+        for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(v[c][j], g[j]);
       }
+      amax = max8(amax, v[c]);
     }
+    float ss = f2_hsum(ss2);
     row_reduce<G>(ss, amax);
     const float inv_h = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
     const float s = scale_of(amax * inv_h, p.q_dtype);
     const float k = inv_h / s;
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], k);
+    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
   } else {
-    float amax = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      chunk_f32<XB>(xc[c], p.x_dtype, v[c]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[c][j]));
+      chunk_f32<XT>(xc[c], v[c]);
+      amax = max8(amax, v[c]);
     }
     row_reduce<G>(none, amax);
     const float s = scale_of(amax, p.q_dtype);
     const float k = 1.0f / s;
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], k);
+    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
   }
 }
 
