@@ -5,12 +5,14 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libglypr_cuda.so")
-SOURCES = ["glypr_cuda.cu", "operators.cu", "gguf.cpp", "engine.cpp", "tokenizer.cpp"]
+SOURCES = ["glypr_cuda.cu", "op_rows.cu", "op_linear.cu", "gguf.cpp", "engine.cpp", "tokenizer.cpp"]
 HEADERS = ["common.cuh", "gemm.cuh", "q8gemm.cuh", "attention_tc.cuh", "attention_d512.cuh", "attention_pair.cuh", "rowops.cuh", "gguf.h", "ple.cuh",
            "rowquant.cuh", "linear.cuh", "linear_any.cuh",
            "linear_tc.cuh", "operators.h", "unicode_case.inc"]
@@ -23,14 +25,16 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def command(extra=()) -> list:
-    return [
-        nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-        "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC,-O3", "-shared",
-        "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-        *[os.path.join(CSRC, s) for s in SOURCES],
-        "-o", LIB, "-cudart", "static", "-lpthread", "-ldl", "-lrt", *extra,
-    ]
+FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+         "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC,-O3", "-I", os.path.join(ROOT, "include"), "-I", CSRC]
+
+
+def commands(obj_dir, extra=()) -> tuple:
+    """One compile command per source, and the link command."""
+    objs = [os.path.join(obj_dir, s + ".o") for s in SOURCES]
+    compiles = [[nvcc(), *FLAGS, "-c", os.path.join(CSRC, s), "-o", o, *extra] for s, o in zip(SOURCES, objs)]
+    return compiles, [nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", *objs, "-o", LIB,
+                      "-cudart", "static", "-lpthread", "-ldl", "-lrt"]
 
 
 def stale() -> bool:
@@ -43,10 +47,16 @@ def stale() -> bool:
 
 def build(force: bool = False, verbose: bool = False, extra=()) -> str:
     if force or stale():
-        cmd = command(extra)
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        with tempfile.TemporaryDirectory() as obj_dir:
+            compiles, link = commands(obj_dir, extra)
+
+            def run(cmd):
+                if verbose:
+                    print(" ".join(cmd), flush=True)
+                subprocess.run(cmd, check=True)
+            with ThreadPoolExecutor(max_workers=min(len(compiles), os.cpu_count() or 1)) as pool:
+                list(pool.map(run, compiles))
+            run(link)
     return LIB
 
 

@@ -1955,7 +1955,7 @@ int noalloc_pointers(int dev, __nv_bfloat16** weight, int** status) {
 
 // ================================================================================= C ABI
 namespace glp {
-// for the engine (engine.cpp) and operators.cu: set the calling thread's glp_last_error() message
+// for engine.cpp and the op_*.cu files: set the calling thread's glp_last_error() message
 void set_last_error(const std::string& msg) { t_err = msg; }
 int kernel_status_word(int dev, int** out) { return device_status_word(dev, out); }
 EncodeTiledFn tensor_map_encoder() { return encode_fn(); }

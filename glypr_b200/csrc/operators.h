@@ -1,8 +1,14 @@
-// What operators.cu takes from the library's core (glypr_cuda.cu).
+// What the translation units of the standalone operators share: the core's services (glypr_cuda.cu),
+// error reporting, argument helpers.
 #pragma once
 #include <cuda.h>
+#include <cuda_runtime.h>
 
+#include <cstdint>
+#include <exception>
 #include <string>
+
+#include "glypr_cuda.h"
 
 namespace glp {
 // the calling thread's glp_last_error() message
@@ -14,4 +20,42 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn tensor_map_encoder();
+
+namespace op {
+
+inline int fail(int code, const char* msg) {
+  set_last_error(msg);
+  return code;
+}
+
+inline int launched(cudaError_t e = cudaGetLastError()) {
+  if (e == cudaSuccess) return GLP_OK;
+  set_last_error(std::string("kernel launch: ") + cudaGetErrorString(e));
+  return e == cudaErrorMemoryAllocation ? GLP_ERR_OOM : GLP_ERR_CUDA;
+}
+
+inline int dtype_size(int dtype) {
+  return dtype == GLP_DTYPE_F32 ? 4 : (dtype == GLP_DTYPE_F16 || dtype == GLP_DTYPE_BF16) ? 2 : 1;
+}
+inline bool wide_dtype(int dtype) { return dtype == GLP_DTYPE_F32 || dtype == GLP_DTYPE_F16 || dtype == GLP_DTYPE_BF16; }
+inline bool code_dtype(int dtype) { return dtype == GLP_DTYPE_I8 || dtype == GLP_DTYPE_E4M3; }
+inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// a row pitch in elements: 0 = packed; false when shorter than the row
+inline bool pitch(int64_t* ld, int64_t cols) {
+  if (*ld == 0) *ld = cols;
+  return *ld >= cols;
+}
+
+// no C++ exception leaves a C entry (an error message is the only allocation)
+template <class F>
+int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception&) {
+    return GLP_ERR_OOM;
+  }
+}
+
+}  // namespace op
 }  // namespace glp
