@@ -78,7 +78,9 @@ __global__ void __launch_bounds__(256) linear_any_kernel(const LinearParams p) {
         if (n >= p.N) continue;
         float v = static_cast<float>(acc[i][j]) * (p.w_scale ? xs * p.w_scale[n] : xs);
         if (p.bias) v += p.bias[n];
-        v = activate(v, p.activation);
+        float pair[2] = {v, v};
+        activate_all(pair, p.activation);
+        v = pair[0];
         if constexpr (GATED) {
           float u = static_cast<float>(up[i][j]) * (p.w_up_scale ? xs * p.w_up_scale[n] : xs);
           if (p.bias_up) u += p.bias_up[n];
