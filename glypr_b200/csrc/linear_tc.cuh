@@ -36,20 +36,25 @@ struct LinearTcParams {
 
 template <int CG, int BN, bool GATED>
 struct LinearTcCfg {
-  static constexpr int OUT_N = GATED ? BN / 2 : BN;       // output columns per tile
-  static constexpr int EPI_WARPS = CG == 2 ? 8 : OUT_N / 16 > 8 ? 8 : OUT_N / 16;
-  static constexpr int W = OUT_N / (EPI_WARPS / 4);       // output columns per epilogue warp
+  static constexpr int OUT_N = GATED ? BN / 2 : BN;  // output columns per tile
+  // 16 epilogue warps where the tile has 32 columns for each: draining a tile is a chain of latencies
+  // (tensor memory, exponentials, the residual), and with 8 warps it took longer than the tile's MMAs
+  // (16,384 x 4,096 x 4,096 e4m3 with erf-GELU: 265 us against 207 us without the drain's work)
+  static constexpr int EPI_WARPS = OUT_N >= 128 ? 16 : OUT_N / 8;
+  static constexpr int W = 4 * OUT_N / EPI_WARPS;    // output columns per epilogue warp
+  static constexpr int CH = GATED ? 16 : 32;         // ... drained at a time (96 registers per thread)
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGES = CG == 2 ? 5 : (BN == 64 ? 6 : 5);
+  static constexpr int STAGES = BN == 64 ? 6 : 4;    // a fifth 32 KB stage changed nothing (178 / 184 us)
   static constexpr uint32_t A_BYTES = 128 * 128;
   static constexpr uint32_t B_ROWS = CG == 2 ? BN / 2 : BN;  // rows of w (and w_up) in this CTA
   static constexpr uint32_t B_BYTES = B_ROWS * 128;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
-  static constexpr uint32_t BOX_OFFSET = STAGES * (A_BYTES + B_BYTES);  // two 4 KB boxes per epilogue warp
-  static constexpr uint32_t COL_OFFSET = BOX_OFFSET + EPI_WARPS * 8192;  // f32 [scale | bias][BN]
-  static constexpr uint32_t BAR_OFFSET = COL_OFFSET + 2 * BN * 4;
+  static constexpr uint32_t BOX_OFFSET = STAGES * (A_BYTES + B_BYTES);  // one 4 KB box per epilogue warp
+  static constexpr uint32_t COL_OFFSET = BOX_OFFSET + EPI_WARPS * 4096;  // f32 [buffer][scale | bias][BN]
+  static constexpr uint32_t BAR_OFFSET = COL_OFFSET + 4 * BN * 4;
   static constexpr size_t SMEM = BAR_OFFSET + 512;
-  static_assert(W == 64 || W == 128, "64 or 128 output columns per warp");
+  static_assert(W == 32 || W == 64, "32 or 64 output columns per warp");
+  static_assert(32 * EPI_WARPS >= BN, "a thread per accumulator column");
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
@@ -71,21 +76,37 @@ __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint
 #undef GLP_UMMA
 }
 
-// bulk stores of this thread but the newest have read their shared memory
-__device__ __forceinline__ void bulk_wait_read_but1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
-
 template <int THREADS>
 __device__ __forceinline__ void epilogue_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
-// 32 accumulator columns -> x w^T xs ws + b, on packed f32 pairs
-template <int KIND>
-__device__ __forceinline__ void scale_bias(const uint32_t (&r)[32], float xs, const float* sw, const float* sb,
-                                           float (&v)[32]) {
+// 16 / 32 consecutive accumulator columns, and the wait for one or two such loads that also names their
+// registers, so that no use of them is scheduled before it
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) { tmem_ld_wait_tied(r); }
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// accumulator columns -> x w^T xs ws + b, on packed f32 pairs
+template <int KIND, int N>
+__device__ __forceinline__ void scale_bias(const uint32_t (&r)[N], float xs, const float* sw, const float* sb,
+                                           float (&v)[N]) {
   const uint64_t xs2 = f2(xs, xs);
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < N; j += 4) {
     const float4 w = *reinterpret_cast<const float4*>(sw + j), b = *reinterpret_cast<const float4*>(sb + j);
     float a[4];
 #pragma unroll
@@ -110,15 +131,13 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
   }
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * Cfg::A_BYTES;
-  float* col_scale = reinterpret_cast<float*>(smem + Cfg::COL_OFFSET);
-  float* col_bias = col_scale + BN;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFFSET);  // of a pair: used in the leader
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;  // a pair's leader: its warps + 1 arrive forwarded from the peer
   uint64_t* drain = tempty + 2;
-  uint64_t* rbar = drain + 1;    // [EPI_WARPS][2] residual boxes
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar + 2 * Cfg::EPI_WARPS);
+  uint64_t* rbar = drain + 1;    // [EPI_WARPS] residual boxes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(rbar + Cfg::EPI_WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* never = abort_flag + 1;  // 0: for the waits that an abort must not cut short
 
@@ -139,7 +158,7 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
       mbar_init(&tempty[b], Cfg::EPI_WARPS + (CG == 2 && leader ? 1 : 0));
     }
     mbar_init(drain, 1);
-    for (int i = 0; i < 2 * Cfg::EPI_WARPS; ++i) mbar_init(&rbar[i], 1);
+    for (int i = 0; i < Cfg::EPI_WARPS; ++i) mbar_init(&rbar[i], 1);
     *abort_flag = 0;
     *never = 0;
     fence_barrier_init();
@@ -288,17 +307,20 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
     }
   } else {
     // -------------------------------------------------------------- epilogue warps
+    constexpr int W = Cfg::W, CH = Cfg::CH;
     const LinearParams& a = p.a;
     const int ew = warp - 2, et = threadIdx.x - 64;
     const int quad = warp & 3;  // the tensor memory lanes that this warp can read
-    const int wcol = (ew >> 2) * Cfg::W;
-    uint8_t* box = smem + Cfg::BOX_OFFSET + ew * 8192;
-    uint64_t* rb = rbar + 2 * ew;
+    const int wcol = (ew >> 2) * W;
+    uint8_t* box = smem + Cfg::BOX_OFFSET + ew * 4096;
+    uint64_t* rb = rbar + ew;
     const bool out16 = a.out_dtype != kF32;
     const bool res_tma = p.tma_out && a.residual;
-    const int slice_cols = out16 ? 64 : 32;  // output columns per box
-    uint32_t rph = 0;  // phase bits of the two residual boxes
-    int turn = 0;      // slices so far: slice i of a tile goes through box (turn + i) & 1
+    const int slice_cols = out16 ? W : 32;  // output columns per box: rows of 128 (16-bit, W = 32: 64) bytes
+    // 16-byte chunk q of this lane's row: the swizzle of the box's tensor map
+    const uint32_t row_bytes = out16 ? W * 2 : 128;
+    const uint32_t row_at = lane * row_bytes, row_swz = row_bytes == 128 ? lane & 7 : (lane >> 1) & 3;
+    uint32_t rph = 0;
     int ab = 0;
     uint32_t aph = 0;
     bool ok = true;
@@ -309,91 +331,85 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
       const int row = wrow0 + lane;
       const int col0 = n_blk * Cfg::OUT_N + wcol;
       // output columns of this warp inside N, none when its rows are past M
-      const int cols = wrow0 < a.M ? max(0, min(Cfg::W, a.N - col0)) : 0;
-      // scale and bias of accumulator column et; of this thread's row
-      float cs = 1.0f, cb = 0.0f;
+      const int cols = wrow0 < a.M ? max(0, min(W, a.N - col0)) : 0;
+      if (res_tma && lane == 0 && cols > 0 && ok) {
+        bulk_wait_read_all();  // the previous tile's outputs have left the box
+        mbar_arrive_expect_tx(rb, 32 * row_bytes);
+        tma_load_2d(box, &tm_r, rb, col0, wrow0);
+      }
+      // scale and bias of accumulator column et, in the buffer that was last read two tiles ago: a warp
+      // passes this sync only when every warp has finished the tile before
+      float* col_scale = reinterpret_cast<float*>(smem + Cfg::COL_OFFSET) + ab * 2 * BN;
+      float* col_bias = col_scale + BN;
       if (et < BN) {
         const bool up = GATED && et >= BN / 2;
         const int n = n_blk * Cfg::OUT_N + (up ? et - BN / 2 : et);
         const float* ws = up ? a.w_up_scale : a.w_scale;
         const float* bs = up ? a.bias_up : a.bias;
-        if (n < a.N) {
-          if (ws) cs = ws[n];
-          if (bs) cb = bs[n];
-        }
+        col_scale[et] = ws && n < a.N ? ws[n] : 1.0f;
+        col_bias[et] = bs && n < a.N ? bs[n] : 0.0f;
       }
       const float xs = a.x_scale && row < a.M ? a.x_scale[row] : 1.0f;
-      epilogue_sync<32 * Cfg::EPI_WARPS>();  // the previous tile's values have been read
-      if (et < BN) {
-        col_scale[et] = cs;
-        col_bias[et] = cb;
-      }
       epilogue_sync<32 * Cfg::EPI_WARPS>();
-      const int slices = (cols + slice_cols - 1) / slice_cols;
-      if (res_tma && lane == 0 && slices > 0 && ok) {
-        bulk_wait_read_all();
-        for (int i = 0; i < min(slices, 2); ++i) {
-          const int b = (turn + i) & 1;
-          mbar_arrive_expect_tx(&rb[b], 4096);
-          tma_load_2d(box + b * 4096, &tm_r, &rb[b], col0 + i * slice_cols, wrow0);
-        }
-      }
-      const int loaded = res_tma && ok ? min(slices, 2) : 0;
+      const bool was_ok = ok;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&tfull[ab], aph, abort_flag));
       if (!ok) {
         if (lane == 0) {
           record_error(a.status, kErrTimeoutEpilogue);
           *abort_flag = 1;
-          for (int i = 0; i < loaded; ++i) mbar_wait(&rb[(turn + i) & 1], (rph >> ((turn + i) & 1)) & 1u, never);
+          if (res_tma && cols > 0 && was_ok) mbar_wait(rb, rph, never);
         }
         continue;
       }
       tc_fence_after();
-      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(ab * BN);
+      const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(ab * BN + wcol);
+      const auto release = [&] {  // this warp has read its part of the accumulator
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tempty[ab]);
+      };
+      if (cols == 0) release();
 #pragma unroll 1
-      for (int c = 0; c < Cfg::W; c += 32) {
-        if (c >= cols) break;
-        float v[32];
+      for (int c = 0; c < cols; c += CH) {
+        float v[CH];
         {
-          uint32_t r[32];
-          tmem_ld32(tacc + wcol + c, r);
+          uint32_t r[CH];
+          tmem_load(tacc + c, r);
           if constexpr (GATED) {
-            uint32_t u[32];
-            float vu[32];
-            tmem_ld32(tacc + BN / 2 + wcol + c, u);
-            tmem_ld_wait_tied(r);
-            tmem_ld_wait_tied(u);
+            uint32_t u[CH];
+            tmem_load(tacc + BN / 2 + c, u);
+            tmem_wait(r);
+            tmem_wait(u);
+            if (c + CH >= cols) release();
+            float vu[CH];
             scale_bias<KIND>(r, xs, col_scale + wcol + c, col_bias + wcol + c, v);
             activate_all(v, a.activation);
             scale_bias<KIND>(u, xs, col_scale + BN / 2 + wcol + c, col_bias + BN / 2 + wcol + c, vu);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= vu[j];
+            for (int j = 0; j < CH; ++j) v[j] *= vu[j];
           } else {
-            tmem_ld_wait_tied(r);
+            tmem_wait(r);
+            if (c + CH >= cols) release();
             scale_bias<KIND>(r, xs, col_scale + wcol + c, col_bias + wcol + c, v);
             activate_all(v, a.activation);
           }
         }
         if (p.tma_out) {
-          const int slice = c / slice_cols, b = (turn + slice) & 1;
-          uint8_t* bx = box + b * 4096;
-          const bool first = c % slice_cols == 0;
-          const bool last = c + 32 >= cols || (c + 32) % slice_cols == 0;
-          if (first) {
+          const int in_slice = c % slice_cols;
+          if (in_slice == 0) {  // the box: holding the residual, or free
             if (res_tma) {
-              ok = __all_sync(0xffffffffu, mbar_wait(&rb[b], (rph >> b) & 1u, never));
-              rph ^= 1u << b;
+              ok = __all_sync(0xffffffffu, mbar_wait(rb, rph, never));
+              rph ^= 1u;
               if (!ok) break;
             } else {
-              if (lane == 0) bulk_wait_read_but1();
+              if (lane == 0) bulk_wait_read_all();
               __syncwarp();
             }
           }
           if (out16) {
-            const int q0 = (c % 64) / 8;  // first of this half's four 16-byte chunks
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4* at = reinterpret_cast<uint4*>(bx + lane * 128 + (((q0 + q) ^ (lane & 7)) << 4));
+            for (int q = 0; q < CH / 8; ++q) {
+              uint4* at = reinterpret_cast<uint4*>(box + row_at + (((in_slice / 8 + q) ^ row_swz) << 4));
               uint32_t w[4];
               if (res_tma) {
                 const uint4 o = *at;
@@ -412,38 +428,39 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
             }
           } else {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              float4* at = reinterpret_cast<float4*>(bx + lane * 128 + ((q ^ (lane & 7)) << 4));
-              float4 o = res_tma ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < CH / 4; ++q) {
+              float4* at = reinterpret_cast<float4*>(box + row_at + (((in_slice / 4 + q) ^ row_swz) << 4));
+              const float4 o = res_tma ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
               *at = make_float4(v[4 * q] + o.x, v[4 * q + 1] + o.y, v[4 * q + 2] + o.z, v[4 * q + 3] + o.w);
             }
           }
-          if (last) {
+          if (c + CH >= cols || in_slice + CH == slice_cols) {
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_2d(&tm_y, bx, col0 + slice * slice_cols, wrow0);
+              const int slice0 = col0 + c - in_slice;
+              tma_store_2d(&tm_y, box, slice0, wrow0);
               bulk_commit();
-              if (res_tma && slice + 2 < slices) {
+              if (res_tma && c + CH < cols) {  // f32 rows of 64 columns take the box twice
                 bulk_wait_read_all();
-                mbar_arrive_expect_tx(&rb[b], 4096);
-                tma_load_2d(bx, &tm_r, &rb[b], col0 + (slice + 2) * slice_cols, wrow0);
+                mbar_arrive_expect_tx(rb, 32 * row_bytes);
+                tma_load_2d(box, &tm_r, rb, slice0 + slice_cols, wrow0);
               }
             }
           }
         } else {
           __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
+          for (int q = 0; q < CH / 4; ++q)
             *reinterpret_cast<float4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) =
                 make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           __syncwarp();
-          const int n = col0 + c + lane;
-          if (c + lane < cols) {
+          const int j = lane % CH, n = col0 + c + j;
+          if (c + j < cols) {
             const int rows = min(32, a.M - wrow0);
-#pragma unroll 8
-            for (int i = 0; i < rows; ++i) {
-              float o = *reinterpret_cast<const float*>(box + i * 128 + ((((lane >> 2) ^ (i & 7)) << 4) | ((lane & 3) << 2)));
+#pragma unroll 4
+            for (int i = lane / CH; i < rows; i += 32 / CH) {
+              float o = *reinterpret_cast<const float*>(box + i * 128 + ((((j >> 2) ^ (i & 7)) << 4) | ((j & 3) << 2)));
               const int64_t m = wrow0 + i;
               if (a.residual) o += load_as_f32(a.residual, m * a.ld_residual + n, a.out_dtype);
               store_from_f32(a.y, m * a.ld_y + n, a.out_dtype, o);
@@ -458,10 +475,6 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
         }
         continue;
       }
-      turn += slices;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[ab]);
       ab ^= 1;
       if (ab == 0) aph ^= 1;
     }

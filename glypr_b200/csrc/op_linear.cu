@@ -26,9 +26,10 @@ int launch_any(const LinearParams& p, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------ tensor-core product
-// a row-major [rows, cols] matrix in boxes of box_rows rows x 128 bytes, 128-byte swizzle, zeros
-// outside.  Encoded on every call: a map is a function of these arguments alone.
-int make_map(CUtensorMap* m, const void* base, int dtype, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+// a row-major [rows, cols] matrix in boxes of box_rows rows x 128 or 64 bytes, swizzled by as many,
+// zeros outside.  Encoded on every call: a map is a function of these arguments alone.
+int make_map(CUtensorMap* m, const void* base, int dtype, int64_t rows, int64_t cols, int64_t ld, int box_rows,
+             int box_bytes = 128) {
   const glp::EncodeTiledFn fn = glp::tensor_map_encoder();
   if (!fn) return fail(GLP_ERR_CUDA, "cuTensorMapEncodeTiled unavailable (driver too old?)");
   const int size = dtype_size(dtype);
@@ -37,10 +38,11 @@ int make_map(CUtensorMap* m, const void* base, int dtype, int64_t rows, int64_t 
                                                : CU_TENSOR_MAP_DATA_TYPE_UINT16;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * size)};
-  const cuuint32_t box[2] = {128u / size, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes / size), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1u, 1u};
   const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return GLP_OK;
   glp::set_last_error("cuTensorMapEncodeTiled failed: " + std::to_string(r));
@@ -101,9 +103,10 @@ int launch_tc(glp::LinearTcParams p, const DeviceInfo& d, cudaStream_t st) {
   if (GATED)
     if (int rc = make_map(&mu, a.w_up, a.dtype, a.N, a.K, a.ld_w, w_rows)) return rc;
   if (p.tma_out) {
-    if (int rc = make_map(&my, a.y, a.out_dtype, a.M, a.N, a.ld_y, 32)) return rc;
+    const int out_bytes = os == 2 && Cfg::W == 32 ? 64 : 128;
+    if (int rc = make_map(&my, a.y, a.out_dtype, a.M, a.N, a.ld_y, 32, out_bytes)) return rc;
     if (a.residual)
-      if (int rc = make_map(&mr, a.residual, a.out_dtype, a.M, a.N, a.ld_residual, 32)) return rc;
+      if (int rc = make_map(&mr, a.residual, a.out_dtype, a.M, a.N, a.ld_residual, 32, out_bytes)) return rc;
   }
   const int units = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.m_tiles) * p.n_tiles, d.sms / CG));
   cudaLaunchConfig_t cfg{};
