@@ -37,24 +37,22 @@ struct LinearTcParams {
 template <int CG, int BN, bool GATED>
 struct LinearTcCfg {
   static constexpr int OUT_N = GATED ? BN / 2 : BN;  // output columns per tile
-  // 16 epilogue warps where the tile has 32 columns for each: draining a tile is a chain of latencies
-  // (tensor memory, exponentials, the residual), and with 8 warps it took longer than the tile's MMAs
-  // (16,384 x 4,096 x 4,096 e4m3 with erf-GELU: 265 us against 207 us without the drain's work)
-  static constexpr int EPI_WARPS = OUT_N >= 128 ? 16 : OUT_N / 8;
+  static constexpr int EPI_WARPS = 8;
   static constexpr int W = 4 * OUT_N / EPI_WARPS;    // output columns per epilogue warp
-  static constexpr int CH = GATED ? 16 : 32;         // ... drained at a time (96 registers per thread)
+  static constexpr int CH = 32;                      // ... drained at a time
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGES = BN == 64 ? 6 : 4;    // a fifth 32 KB stage changed nothing (178 / 184 us)
+  static constexpr int STAGES = BN == 64 ? 6 : 5;
   static constexpr uint32_t A_BYTES = 128 * 128;
   static constexpr uint32_t B_ROWS = CG == 2 ? BN / 2 : BN;  // rows of w (and w_up) in this CTA
   static constexpr uint32_t B_BYTES = B_ROWS * 128;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
   static constexpr uint32_t BOX_OFFSET = STAGES * (A_BYTES + B_BYTES);  // one 4 KB box per epilogue warp
-  static constexpr uint32_t COL_OFFSET = BOX_OFFSET + EPI_WARPS * 4096;  // f32 [buffer][scale | bias][BN]
-  static constexpr uint32_t BAR_OFFSET = COL_OFFSET + 4 * BN * 4;
+  // f32 [scale | bias | scale of w_up | bias_up][W] per epilogue warp
+  static constexpr uint32_t COL_OFFSET = BOX_OFFSET + EPI_WARPS * 4096;
+  static constexpr uint32_t COL_BYTES = (GATED ? 4 : 2) * W * 4;
+  static constexpr uint32_t BAR_OFFSET = COL_OFFSET + EPI_WARPS * COL_BYTES;
   static constexpr size_t SMEM = BAR_OFFSET + 512;
-  static_assert(W == 32 || W == 64, "32 or 64 output columns per warp");
-  static_assert(32 * EPI_WARPS >= BN, "a thread per accumulator column");
+  static_assert(W == 32 || W == 64 || W == 128, "whole chunks of columns per warp");
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
@@ -74,11 +72,6 @@ __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint
     if constexpr (KIND == kMmaI8) GLP_UMMA("2", "i8");
   }
 #undef GLP_UMMA
-}
-
-template <int THREADS>
-__device__ __forceinline__ void epilogue_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
 // 16 / 32 consecutive accumulator columns, and the wait for one or two such loads that also names their
@@ -309,22 +302,23 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
     // -------------------------------------------------------------- epilogue warps
     constexpr int W = Cfg::W, CH = Cfg::CH;
     const LinearParams& a = p.a;
-    const int ew = warp - 2, et = threadIdx.x - 64;
+    const int ew = warp - 2;
     const int quad = warp & 3;  // the tensor memory lanes that this warp can read
     const int wcol = (ew >> 2) * W;
     uint8_t* box = smem + Cfg::BOX_OFFSET + ew * 4096;
     uint64_t* rb = rbar + ew;
     const bool out16 = a.out_dtype != kF32;
     const bool res_tma = p.tma_out && a.residual;
-    const int slice_cols = out16 ? W : 32;  // output columns per box: rows of 128 (16-bit, W = 32: 64) bytes
+    float* col = reinterpret_cast<float*>(smem + Cfg::COL_OFFSET + ew * Cfg::COL_BYTES);
+    // output columns per box: rows of 128 (16-bit, W = 32: 64) bytes
+    const int slice_cols = out16 ? (W < 64 ? W : 64) : 32;
     // 16-byte chunk q of this lane's row: the swizzle of the box's tensor map
-    const uint32_t row_bytes = out16 ? W * 2 : 128;
+    const uint32_t row_bytes = out16 ? slice_cols * 2 : 128;
     const uint32_t row_at = lane * row_bytes, row_swz = row_bytes == 128 ? lane & 7 : (lane >> 1) & 3;
     uint32_t rph = 0;
     int ab = 0;
     uint32_t aph = 0;
     bool ok = true;
-    // A warp whose wait ran out still walks every tile, so that no epilogue_sync is left short.
     for (int tile = unit; tile < num_tiles; tile += units) {
       const int m_blk = tile / p.n_tiles, n_blk = tile % p.n_tiles;
       const int wrow0 = (m_blk * CG + static_cast<int>(rank)) * 128 + quad * 32;
@@ -332,34 +326,29 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
       const int col0 = n_blk * Cfg::OUT_N + wcol;
       // output columns of this warp inside N, none when its rows are past M
       const int cols = wrow0 < a.M ? max(0, min(W, a.N - col0)) : 0;
-      if (res_tma && lane == 0 && cols > 0 && ok) {
+      if (res_tma && lane == 0 && cols > 0) {
         bulk_wait_read_all();  // the previous tile's outputs have left the box
         mbar_arrive_expect_tx(rb, 32 * row_bytes);
         tma_load_2d(box, &tm_r, rb, col0, wrow0);
       }
-      // scale and bias of accumulator column et, in the buffer that was last read two tiles ago: a warp
-      // passes this sync only when every warp has finished the tile before
-      float* col_scale = reinterpret_cast<float*>(smem + Cfg::COL_OFFSET) + ab * 2 * BN;
-      float* col_bias = col_scale + BN;
-      if (et < BN) {
-        const bool up = GATED && et >= BN / 2;
-        const int n = n_blk * Cfg::OUT_N + (up ? et - BN / 2 : et);
-        const float* ws = up ? a.w_up_scale : a.w_scale;
-        const float* bs = up ? a.bias_up : a.bias;
-        col_scale[et] = ws && n < a.N ? ws[n] : 1.0f;
-        col_bias[et] = bs && n < a.N ? bs[n] : 0.0f;
+      // scales and biases of this warp's columns, and of this lane's row
+#pragma unroll
+      for (int j = 0; j < W; j += 32) {
+        const int n = col0 + j + lane;
+        const bool in = n < a.N;
+        col[j + lane] = a.w_scale && in ? a.w_scale[n] : 1.0f;
+        col[W + j + lane] = a.bias && in ? a.bias[n] : 0.0f;
+        if constexpr (GATED) {
+          col[2 * W + j + lane] = a.w_up_scale && in ? a.w_up_scale[n] : 1.0f;
+          col[3 * W + j + lane] = a.bias_up && in ? a.bias_up[n] : 0.0f;
+        }
       }
       const float xs = a.x_scale && row < a.M ? a.x_scale[row] : 1.0f;
-      epilogue_sync<32 * Cfg::EPI_WARPS>();
-      const bool was_ok = ok;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&tfull[ab], aph, abort_flag));
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, mbar_wait(&tfull[ab], aph, abort_flag));
       if (!ok) {
-        if (lane == 0) {
-          record_error(a.status, kErrTimeoutEpilogue);
-          *abort_flag = 1;
-          if (res_tma && cols > 0 && was_ok) mbar_wait(rb, rph, never);
-        }
-        continue;
+        if (lane == 0 && res_tma && cols > 0) mbar_wait(rb, rph, never);
+        break;
       }
       tc_fence_after();
       const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(ab * BN + wcol);
@@ -382,15 +371,15 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
             tmem_wait(u);
             if (c + CH >= cols) release();
             float vu[CH];
-            scale_bias<KIND>(r, xs, col_scale + wcol + c, col_bias + wcol + c, v);
+            scale_bias<KIND>(r, xs, col + c, col + W + c, v);
             activate_all(v, a.activation);
-            scale_bias<KIND>(u, xs, col_scale + BN / 2 + wcol + c, col_bias + BN / 2 + wcol + c, vu);
+            scale_bias<KIND>(u, xs, col + 2 * W + c, col + 3 * W + c, vu);
 #pragma unroll
             for (int j = 0; j < CH; ++j) v[j] *= vu[j];
           } else {
             tmem_wait(r);
             if (c + CH >= cols) release();
-            scale_bias<KIND>(r, xs, col_scale + wcol + c, col_bias + wcol + c, v);
+            scale_bias<KIND>(r, xs, col + c, col + W + c, v);
             activate_all(v, a.activation);
           }
         }
@@ -468,15 +457,14 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
           }
         }
       }
-      if (!ok) {
-        if (lane == 0) {
-          record_error(a.status, kErrTimeoutEpilogue);
-          *abort_flag = 1;
-        }
-        continue;
-      }
+      if (!ok) break;
+      __syncwarp();  // the columns' values have been read
       ab ^= 1;
       if (ab == 0) aph ^= 1;
+    }
+    if (!ok && lane == 0) {
+      record_error(a.status, kErrTimeoutEpilogue);
+      *abort_flag = 1;
     }
     if (lane == 0) bulk_wait_all();  // this warp's stores are in global memory
   }
