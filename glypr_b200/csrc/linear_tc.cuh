@@ -34,14 +34,14 @@ struct LinearTcParams {
   int tma_out;      // y (and residual) go by bulk copies
 };
 
-template <int CG, int BN, bool GATED>
+template <int CG, int BN, bool GATED, int EPI>
 struct LinearTcCfg {
   static constexpr int OUT_N = GATED ? BN / 2 : BN;  // output columns per tile
-  static constexpr int EPI_WARPS = 8;
-  static constexpr int W = 4 * OUT_N / EPI_WARPS;    // output columns per epilogue warp
-  static constexpr int CH = 32;                      // ... drained at a time
+  static constexpr int EPI_WARPS = EPI;
+  static constexpr int W = 4 * OUT_N / EPI;          // output columns per epilogue warp
+  static constexpr int CH = GATED && EPI == 16 ? 16 : 32;   // ... drained at a time
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGES = BN == 64 ? 6 : 5;
+  static constexpr int STAGES = BN == 64 ? 6 : (EPI == 16 ? 4 : 5);
   static constexpr uint32_t A_BYTES = 128 * 128;
   static constexpr uint32_t B_ROWS = CG == 2 ? BN / 2 : BN;  // rows of w (and w_up) in this CTA
   static constexpr uint32_t B_BYTES = B_ROWS * 128;
@@ -109,12 +109,12 @@ __device__ __forceinline__ void scale_bias(const uint32_t (&r)[N], float xs, con
   }
 }
 
-template <int KIND, int CG, int BN, bool GATED>
-__global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED>::THREADS, 1)
+template <int KIND, int CG, int BN, bool GATED, int EPI>
+__global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED, EPI>::THREADS, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                      const __grid_constant__ CUtensorMap tm_u, const __grid_constant__ CUtensorMap tm_r,
                      const __grid_constant__ CUtensorMap tm_y, const LinearTcParams p) {
-  using Cfg = LinearTcCfg<CG, BN, GATED>;
+  using Cfg = LinearTcCfg<CG, BN, GATED, EPI>;
   constexpr int STAGES = Cfg::STAGES;
   extern __shared__ __align__(1024) uint8_t smem[];
   // (the same for both CTAs of a pair, so both leave before any cluster-wide step)
