@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from typing import List, Optional, Sequence, Union
 
@@ -88,22 +89,10 @@ class GlpTiming(ctypes.Structure):
     _fields_ = [("n_devices", ctypes.c_int), ("device_ms", ctypes.c_float * GLP_MAX_DEVICES)]
 
 
-class GlpNormQ8Args(ctypes.Structure):
-    _fields_ = ([("M", ctypes.c_int), ("H", ctypes.c_int), ("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64),
-                 ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64), ("post_gain", ctypes.c_void_p),
-                 ("gain", ctypes.c_void_p), ("eps", ctypes.c_float), ("layer_scalar", ctypes.c_float),
-                 ("h", ctypes.c_void_p), ("ld_h", ctypes.c_int64), ("q", ctypes.c_void_p), ("ld_q", ctypes.c_int64),
-                 ("scale", ctypes.c_void_p)]
-                + [(n, ctypes.c_int) for n in ("x_dtype", "h_dtype", "q_dtype")])
-
-
-class GlpLinearArgs(ctypes.Structure):
-    _fields_ = ([(n, ctypes.c_int) for n in ("M", "N", "K", "dtype")]
-                + [("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64), ("w", ctypes.c_void_p),
-                   ("w_up", ctypes.c_void_p), ("ld_w", ctypes.c_int64)]
-                + [(n, ctypes.c_void_p) for n in ("x_scale", "w_scale", "w_up_scale", "bias", "bias_up", "residual")]
-                + [("ld_residual", ctypes.c_int64), ("y", ctypes.c_void_p), ("ld_y", ctypes.c_int64),
-                   ("out_dtype", ctypes.c_int), ("activation", ctypes.c_int)])
+# glp_norm_q8_args and glp_linear_args as packed bytes (native layout): a fraction of the time that
+# filling a ctypes.Structure takes, which a single-token call would feel
+_NORM_Q8_ARGS = struct.Struct("@iiPqPqPPffPqPqPiii4x")
+_LINEAR_ARGS = struct.Struct("@iiiiPqPPqPPPPPPqPqii")
 
 
 class GlpProfile(ctypes.Structure):
@@ -181,9 +170,9 @@ def load_library(path: Optional[str] = None) -> ctypes.CDLL:
         L.glp_selftest_wait_timeout.argtypes = [I, I]
         L.glp_gate_up_geglu.argtypes = [P, P, I, I, P, I, P, P]
         L.glp_qkv_norm_rope.argtypes = [P, I, I, I, P, I, P, P, P, ctypes.c_double, I, ctypes.c_float, P, P]
-        L.glp_norm_residual_q8.argtypes = [P, P]
+        L.glp_norm_residual_q8.argtypes = [ctypes.c_char_p, P]
         L.glp_quantize_rows.argtypes = [P, I, I64, I, I, P, I, I64, P, P]
-        L.glp_linear.argtypes = [P, P]
+        L.glp_linear.argtypes = [ctypes.c_char_p, P]
         _lib = L
         return L
 
@@ -478,15 +467,19 @@ def norm_residual_q8(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dty
                      ld_q: int = 0, stream: int = 0) -> None:
     """glp_norm_residual_q8: h = (residual + x~) * layer_scalar and the 8-bit form of RMSNorm(h) * gain.
     Device pointers as ints (0 = not given), types from ``DTYPES``, pitches in elements (0 = packed)."""
-    a = GlpNormQ8Args(m, h_len, d_x, ld_x, residual, ld_residual, post_gain, gain, eps, layer_scalar, h, ld_h, d_q,
-                      ld_q, d_scale, x_dtype, h_dtype, q_dtype)
-    check((_lib or load_library()).glp_norm_residual_q8(ctypes.byref(a), stream))
+    rc = (_lib or load_library()).glp_norm_residual_q8(
+        _NORM_Q8_ARGS.pack(m, h_len, d_x, ld_x, residual, ld_residual, post_gain, gain, eps, layer_scalar, h, ld_h, d_q,
+                           ld_q, d_scale, x_dtype, h_dtype, q_dtype), stream)
+    if rc:
+        check(rc)
 
 
 def quantize_rows(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dtype: int, d_scale: int, *,
                   ld_x: int = 0, ld_q: int = 0, stream: int = 0) -> None:
     """glp_quantize_rows: the 8-bit form (codes and one scale per row) of x [m, h_len]."""
-    check((_lib or load_library()).glp_quantize_rows(d_x, x_dtype, ld_x, m, h_len, d_q, q_dtype, ld_q, d_scale, stream))
+    rc = (_lib or load_library()).glp_quantize_rows(d_x, x_dtype, ld_x, m, h_len, d_q, q_dtype, ld_q, d_scale, stream)
+    if rc:
+        check(rc)
 
 
 def linear(m: int, n: int, k: int, dtype: int, d_x: int, d_w: int, d_y: int, out_dtype: int, *, x_scale: int = 0,
@@ -496,9 +489,11 @@ def linear(m: int, n: int, k: int, dtype: int, d_x: int, d_w: int, d_y: int, out
     """glp_linear: y = act(x w^T * scales + bias) [* (x w_up^T * scales + bias_up)] + residual.
     Device pointers as ints (0 = not given), types from ``DTYPES``, ``activation`` from
     ``ACTIVATIONS``, pitches in elements (0 = packed)."""
-    a = GlpLinearArgs(m, n, k, dtype, d_x, ldx, d_w, w_up, ldw, x_scale, w_scale, w_up_scale, bias, bias_up, residual,
-                      ld_residual, d_y, ldy, out_dtype, activation)
-    check((_lib or load_library()).glp_linear(ctypes.byref(a), stream))
+    rc = (_lib or load_library()).glp_linear(
+        _LINEAR_ARGS.pack(m, n, k, dtype, d_x, ldx, d_w, w_up, ldw, x_scale, w_scale, w_up_scale, bias, bias_up, residual,
+                          ld_residual, d_y, ldy, out_dtype, activation), stream)
+    if rc:
+        check(rc)
 
 
 def flash_attention(d_qkv: int, d_cu: int, n_seq: int, max_len: int, n_q_heads: int, n_kv_heads: int,

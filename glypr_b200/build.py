@@ -15,7 +15,7 @@ LIB = os.path.join(HERE, "libglypr_cuda.so")
 SOURCES = ["glypr_cuda.cu", "op_rows.cu", "op_linear.cu", "gguf.cpp", "engine.cpp", "tokenizer.cpp"]
 HEADERS = ["common.cuh", "gemm.cuh", "q8gemm.cuh", "attention_tc.cuh", "attention_d512.cuh", "attention_pair.cuh", "rowops.cuh", "gguf.h", "ple.cuh",
            "rowquant.cuh", "linear.cuh", "linear_any.cuh",
-           "linear_tc.cuh", "operators.h", "unicode_case.inc"]
+           "linear_rows.cuh", "linear_tc.cuh", "operators.h", "unicode_case.inc"]
 
 
 def nvcc() -> str:

@@ -3,6 +3,7 @@
 #include <atomic>
 
 #include "linear_any.cuh"
+#include "linear_rows.cuh"
 #include "linear_tc.cuh"
 #include "operators.h"
 
@@ -143,6 +144,44 @@ int launch_tc_kind(const LinearParams& a, const DeviceInfo& d, cudaStream_t st) 
   return launch_tc<KIND, 1, 64, false>(p, d, st);
 }
 
+// ------------------------------------------------------------------------------ few rows
+template <int DT, bool GATED, int MT, int R, int U, int WARPS>
+int launch_rows(const LinearParams& p, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>((p.N + 8ll * R - 1) / (8 * R));
+  glp::linear_rows_kernel<DT, GATED, MT, R, U, WARPS><<<grid, 32 * WARPS, 0, st>>>(p);
+  return launched();
+}
+
+// Whether the few-rows kernel is the faster one: always up to 16 rows.  Its blocks each read x again, so
+// with more rows only while that stays small: M = 64, 768 x 768 f16 4.9 us (tensor-memory kernel 7.3 us,
+// 9 MB of x read), 4,096 x 4,096 f16 31 us (22 us, 268 MB).  Up to 32 rows also where the weights have
+// too few rows for the other kernel's 64-wide tiles to fill the device (4,096 x 4,096 f16: 12 us, 22 us;
+// 8,191 x 4,096 e4m3: 20 us, 15 us).
+bool few_rows(const LinearParams& p, const DeviceInfo& d) {
+  if (p.M <= 16) return true;
+  if (p.M > 64) return false;
+  const int64_t x_traffic = (p.N + 7ll) / 8 * p.M * p.K * dtype_size(p.dtype);
+  return x_traffic <= (32 << 20) || (p.M <= 32 && p.N < 48 * d.sms);
+}
+
+// R: 8 rows of w per block while those blocks fit the device at once, 16 beyond (4,096 x 4,096 f16, one row:
+// 9.8 us with 8, 7.3 us with 16; 768 x 768: 2.4 / 2.6 us).
+template <int DT, bool GATED>
+int launch_rows(const LinearParams& p, const DeviceInfo& d, cudaStream_t st) {
+  if (p.M <= 16)
+    return p.N <= 16 * d.sms ? launch_rows<DT, GATED, 1, 1, 2, 16>(p, st) : launch_rows<DT, GATED, 1, 2, 2, 16>(p, st);
+  if (p.M <= 32) {
+    if (GATED) return launch_rows<DT, GATED, 2, 1, 1, 16>(p, st);
+    return p.N <= 8 * d.sms ? launch_rows<DT, GATED, 2, 1, 2, 16>(p, st) : launch_rows<DT, GATED, 2, GATED ? 1 : 2, 1, 16>(p, st);
+  }
+  return launch_rows<DT, GATED, 4, 1, 1, GATED ? 8 : 16>(p, st);  // gated: sums of 16 warps would not fit
+}
+
+template <int DT>
+int launch_rows(const LinearParams& p, const DeviceInfo& d, cudaStream_t st) {
+  return p.w_up ? launch_rows<DT, true>(p, d, st) : launch_rows<DT, false>(p, d, st);
+}
+
 bool tc_operands(const LinearParams& p) {
   const size_t es = dtype_size(p.dtype);
   return aligned(p.x, 16) && aligned(p.w, 16) && aligned(p.w_up, 16) && p.ld_x * es % 16 == 0 && p.ld_w * es % 16 == 0;
@@ -181,6 +220,14 @@ int linear(const glp_linear_args* a, cudaStream_t st) {
   if (tc_operands(p)) {
     DeviceInfo d;
     if (int rc = device_info(&d)) return rc;
+    if (few_rows(p, d)) {
+      switch (p.dtype) {
+        case GLP_DTYPE_F16: return launch_rows<glp::kF16>(p, d, st);
+        case GLP_DTYPE_BF16: return launch_rows<glp::kBF16>(p, d, st);
+        case GLP_DTYPE_I8: return launch_rows<glp::kI8>(p, d, st);
+        default: return launch_rows<glp::kE4M3>(p, d, st);
+      }
+    }
     if (p.dtype == GLP_DTYPE_I8) return launch_tc_kind<glp::kMmaI8>(p, d, st);
     if (p.dtype == GLP_DTYPE_E4M3) return launch_tc_kind<glp::kMmaE4M3>(p, d, st);
     return launch_tc_kind<glp::kMmaF16>(p, d, st);
