@@ -109,6 +109,53 @@ __device__ __forceinline__ void scale_bias(const uint32_t (&r)[N], float xs, con
   }
 }
 
+// n of N elements one pitch apart, raw (zeros after the n-th), and back.  The types and the whole column
+// are told apart outside the loops, so that all loads are on their way before the first is used.
+template <int N>
+__device__ __forceinline__ void load_column(const void* base, int64_t at, int64_t pitch, int n, bool is16, uint32_t (&v)[N]) {
+  if (is16) {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (n == N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i, p += pitch) v[i] = *p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i, p += pitch) v[i] = i < n ? *p : 0;
+    }
+  } else {
+    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += pitch) v[i] = i < n ? *p : 0;
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_column(void* base, int64_t at, int64_t pitch, int n, int dtype, const float (&v)[N]) {
+  if (dtype == kF32) {
+    float* p = static_cast<float*>(base) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += pitch)
+      if (i < n) *p = v[i];
+    return;
+  }
+  uint16_t h[N];
+  if (dtype == kF16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = __half_as_ushort(__float2half_rn(v[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
+  }
+  uint16_t* p = static_cast<uint16_t*>(base) + at;
+  if (n == N) {
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += pitch) *p = h[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += pitch)
+      if (i < n) *p = h[i];
+  }
+}
+
 template <int KIND, int CG, int BN, bool GATED, int EPI>
 __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED, EPI>::THREADS, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
@@ -361,6 +408,15 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED, EPI>::THREADS, 1)
 #pragma unroll 1
       for (int c = 0; c < cols; c += CH) {
         float v[CH];
+        // y or residual off 16-byte rows: this lane's column of the residual's 32 rows, on its way early
+        constexpr int LROWS = CH;  // 32 rows by 32 / CH lanes per column
+        const int gj = lane % CH, gi = lane / CH;
+        const bool gcol = c + gj < cols;
+        const int grows = min(32, a.M - wrow0);
+        uint32_t res[LROWS];  // raw
+        if (!p.tma_out && a.residual)
+          load_column<LROWS>(a.residual, (wrow0 + static_cast<int64_t>(gi)) * a.ld_residual + col0 + c + gj,
+                             a.ld_residual * (32 / CH), gcol ? (grows - gi + 32 / CH - 1) / (32 / CH) : 0, out16, res);
         {
           uint32_t r[CH];
           tmem_load(tacc + c, r);
@@ -444,17 +500,23 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED, EPI>::THREADS, 1)
             *reinterpret_cast<float4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) =
                 make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
           __syncwarp();
-          const int j = lane % CH, n = col0 + c + j;
-          if (c + j < cols) {
-            const int rows = min(32, a.M - wrow0);
-#pragma unroll 4
-            for (int i = lane / CH; i < rows; i += 32 / CH) {
-              float o = *reinterpret_cast<const float*>(box + i * 128 + ((((j >> 2) ^ (i & 7)) << 4) | ((j & 3) << 2)));
-              const int64_t m = wrow0 + i;
-              if (a.residual) o += load_as_f32(a.residual, m * a.ld_residual + n, a.out_dtype);
-              store_from_f32(a.y, m * a.ld_y + n, a.out_dtype, o);
+          float o[LROWS];
+#pragma unroll
+          for (int i = 0; i < LROWS; ++i) {
+            const int rr = gi + i * (32 / CH);
+            o[i] = *reinterpret_cast<const float*>(box + rr * 128 + ((((gj >> 2) ^ (rr & 7)) << 4) | ((gj & 3) << 2)));
+          }
+          if (a.residual) {
+            if (a.out_dtype == kF16) {
+#pragma unroll
+              for (int i = 0; i < LROWS; ++i) o[i] += __half2float(__ushort_as_half(static_cast<unsigned short>(res[i])));
+            } else {
+#pragma unroll
+              for (int i = 0; i < LROWS; ++i) o[i] += __uint_as_float(out16 ? res[i] << 16 : res[i]);
             }
           }
+          store_column<LROWS>(a.y, (wrow0 + static_cast<int64_t>(gi)) * a.ld_y + col0 + c + gj, a.ld_y * (32 / CH),
+                              gcol ? (grows - gi + 32 / CH - 1) / (32 / CH) : 0, a.out_dtype, o);
         }
       }
       if (!ok) break;

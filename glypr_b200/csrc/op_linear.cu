@@ -130,8 +130,19 @@ int launch_tc_kind(const LinearParams& a, const DeviceInfo& d, cudaStream_t st) 
   p.a = a;
   p.a.status = d.status;
   const bool gated = a.w_up != nullptr;
-  const int64_t rows128 = (a.M + 127) / 128, pairs = ((a.M + 255ll) / 256) * ((a.N + (gated ? 127ll : 255ll)) / (gated ? 128 : 256));
-  if (pairs >= d.sms / 2) {
+  // The tile by estimated time: a fixed part, and per wave of tiles the K steps (128 bytes of a row each)
+  // or, with few of them, the drain.  Microseconds, read off M = 512 .. 16,384 against N x K of 768 x 768
+  // f16, 768 x 1,152 and 2,304 x 768 int8, 4,096 x 4,096 e4m3 with bias and residual, and gated 1,152 x 768
+  // int8; e.g. M = 512, 768 x 768 f16: 64-wide 7.3, 128-wide 8.2, pairs 11.1; M = 4,096: 15.1, 12.9, 11.9.
+  const int steps = (a.K * dtype_size(a.dtype) + 127) / 128;
+  const auto estimate = [&](int64_t rows, int64_t cols, int64_t slots, double fixed, double step, double drain) {
+    const int64_t tiles = ((a.M + rows - 1) / rows) * ((a.N + cols - 1) / cols);
+    return fixed + static_cast<double>((tiles + slots - 1) / slots) * std::max(step * steps, drain);
+  };
+  const double pair = estimate(256, gated ? 128 : 256, d.sms / 2, 5.0, 0.43, gated ? 3.5 : 5.4);
+  const double single128 = estimate(128, gated ? 64 : 128, d.sms, 3.5, 0.37, gated ? 2.5 : 3.15);
+  const double single64 = gated ? 1e30 : estimate(128, 64, d.sms, 3.6, 0.31, 2.0);
+  if (pair <= single128 && pair <= single64) {
     // 16 warps drain a tile whose outputs take two exponentials or reciprocals each: their phases (tensor
     // memory, special functions, stores) then overlap between warps.  131,072 x 2,304 x 768 e4m3 with SiLU:
     // 310 us, 373 us with 8; without an activation 281 us, 279 us with 8, and bf16 227 / 216 us.
@@ -140,8 +151,7 @@ int launch_tc_kind(const LinearParams& a, const DeviceInfo& d, cudaStream_t st) 
     return heavy ? launch_tc<KIND, 2, 256, false, 16>(p, d, st) : launch_tc<KIND, 2, 256, false, 8>(p, d, st);
   }
   if (gated) return launch_tc<KIND, 1, 128, true>(p, d, st);
-  if (rows128 * ((a.N + 127ll) / 128) >= d.sms / 2) return launch_tc<KIND, 1, 128, false>(p, d, st);
-  return launch_tc<KIND, 1, 64, false>(p, d, st);
+  return single128 < single64 ? launch_tc<KIND, 1, 128, false>(p, d, st) : launch_tc<KIND, 1, 64, false>(p, d, st);
 }
 
 // ------------------------------------------------------------------------------ few rows
