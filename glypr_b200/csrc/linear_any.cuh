@@ -33,6 +33,8 @@ template <int DT, bool GATED>
 __global__ void __launch_bounds__(256) linear_any_kernel(const LinearParams p) {
   using T = typename AnyAcc<DT>::T;
   __shared__ T sx[16][65], sw[16][65], su[GATED ? 16 : 1][65];
+  griddep_launch();
+  griddep_wait();
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int64_t n_tiles = (p.N + 63) / 64, tiles = n_tiles * ((p.M + 63) / 64);
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {

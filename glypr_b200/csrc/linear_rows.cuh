@@ -78,6 +78,8 @@ __global__ void __launch_bounds__(32 * WARPS) linear_rows_kernel(const LinearPar
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * COLS;
   const int bytes = p.K * ES, steps = (bytes + 63) / 64;
+  griddep_launch();
+  griddep_wait();
   // what the epilogue needs besides the sums, on its way during the products
   float xs[PER], ws[PER], wus[PER], b[PER], bu[PER], res[PER];
 #pragma unroll

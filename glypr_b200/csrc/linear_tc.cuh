@@ -221,6 +221,8 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED, EPI>::THREADS, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  griddep_launch();
+  griddep_wait();  // before anything in global memory is read or written
 
   if (warp == 0) {
     if (lane == 0) {

@@ -19,11 +19,7 @@ template <int DT>
 int launch_any(const LinearParams& p, cudaStream_t st) {
   const int64_t tiles = ((p.M + 63ll) / 64) * ((p.N + 63ll) / 64);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, 1 << 20));
-  if (p.w_up)
-    glp::linear_any_kernel<DT, true><<<grid, 256, 0, st>>>(p);
-  else
-    glp::linear_any_kernel<DT, false><<<grid, 256, 0, st>>>(p);
-  return launched();
+  return launch(p.w_up ? glp::linear_any_kernel<DT, true> : glp::linear_any_kernel<DT, false>, grid, 256, 0, 1, st, p);
 }
 
 // ------------------------------------------------------------------------------ tensor-core product
@@ -110,18 +106,7 @@ int launch_tc(glp::LinearTcParams p, const DeviceInfo& d, cudaStream_t st) {
       if (int rc = make_map(&mr, a.residual, a.out_dtype, a.M, a.N, a.ld_residual, 32, out_bytes)) return rc;
   }
   const int units = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.m_tiles) * p.n_tiles, d.sms / CG));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
-  cfg.blockDim = dim3(Cfg::THREADS);
-  cfg.dynamicSmemBytes = Cfg::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
-  return launched(cudaLaunchKernelEx(&cfg, kernel, mx, mw, mu, mr, my, p));
+  return launch(kernel, static_cast<unsigned>(units * CG), Cfg::THREADS, Cfg::SMEM, CG, st, mx, mw, mu, mr, my, p);
 }
 
 template <int KIND>
@@ -158,8 +143,7 @@ int launch_tc_kind(const LinearParams& a, const DeviceInfo& d, cudaStream_t st) 
 template <int DT, bool GATED, int MT, int R, int U, int WARPS>
 int launch_rows(const LinearParams& p, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>((p.N + 8ll * R - 1) / (8 * R));
-  glp::linear_rows_kernel<DT, GATED, MT, R, U, WARPS><<<grid, 32 * WARPS, 0, st>>>(p);
-  return launched();
+  return launch(glp::linear_rows_kernel<DT, GATED, MT, R, U, WARPS>, grid, 32 * WARPS, 0, 1, st, p);
 }
 
 // Whether the few-rows kernel is the faster one: always up to 16 rows.  Its blocks each read x again, so

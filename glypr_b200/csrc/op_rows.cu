@@ -18,21 +18,20 @@ int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
   constexpr int ROWS = G == 32 ? 8 : 1;
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.M) + ROWS - 1) / ROWS), block = G == 32 ? 256 : G;
   if constexpr (NORM) {
-    const auto with_h = [&](auto xt) {
+    const auto with_h = [&](auto xt) -> int {
       constexpr int XT = decltype(xt)::value;
-      if (p.h_dtype == GLP_DTYPE_F32) glp::row_quant_kernel<G, NC, XT, glp::kF32, true><<<grid, block, 0, st>>>(p, gains16);
-      if (p.h_dtype == GLP_DTYPE_F16) glp::row_quant_kernel<G, NC, XT, glp::kF16, true><<<grid, block, 0, st>>>(p, gains16);
-      if (p.h_dtype == GLP_DTYPE_BF16) glp::row_quant_kernel<G, NC, XT, glp::kBF16, true><<<grid, block, 0, st>>>(p, gains16);
+      if (p.h_dtype == GLP_DTYPE_F32) return launch(glp::row_quant_kernel<G, NC, XT, glp::kF32, true>, grid, block, 0, 1, st, p, gains16);
+      if (p.h_dtype == GLP_DTYPE_F16) return launch(glp::row_quant_kernel<G, NC, XT, glp::kF16, true>, grid, block, 0, 1, st, p, gains16);
+      return launch(glp::row_quant_kernel<G, NC, XT, glp::kBF16, true>, grid, block, 0, 1, st, p, gains16);
     };
-    if (p.x_dtype == GLP_DTYPE_F32) with_h(std::integral_constant<int, glp::kF32>{});
-    if (p.x_dtype == GLP_DTYPE_F16) with_h(std::integral_constant<int, glp::kF16>{});
-    if (p.x_dtype == GLP_DTYPE_BF16) with_h(std::integral_constant<int, glp::kBF16>{});
+    if (p.x_dtype == GLP_DTYPE_F32) return with_h(std::integral_constant<int, glp::kF32>{});
+    if (p.x_dtype == GLP_DTYPE_F16) return with_h(std::integral_constant<int, glp::kF16>{});
+    return with_h(std::integral_constant<int, glp::kBF16>{});
   } else {
-    if (p.x_dtype == GLP_DTYPE_F32) glp::row_quant_kernel<G, NC, glp::kF32, glp::kF32, false><<<grid, block, 0, st>>>(p, false);
-    if (p.x_dtype == GLP_DTYPE_F16) glp::row_quant_kernel<G, NC, glp::kF16, glp::kF16, false><<<grid, block, 0, st>>>(p, false);
-    if (p.x_dtype == GLP_DTYPE_BF16) glp::row_quant_kernel<G, NC, glp::kBF16, glp::kBF16, false><<<grid, block, 0, st>>>(p, false);
+    if (p.x_dtype == GLP_DTYPE_F32) return launch(glp::row_quant_kernel<G, NC, glp::kF32, glp::kF32, false>, grid, block, 0, 1, st, p, false);
+    if (p.x_dtype == GLP_DTYPE_F16) return launch(glp::row_quant_kernel<G, NC, glp::kF16, glp::kF16, false>, grid, block, 0, 1, st, p, false);
+    return launch(glp::row_quant_kernel<G, NC, glp::kBF16, glp::kBF16, false>, grid, block, 0, 1, st, p, false);
   }
-  return launched();
 }
 
 // Whether every row's x, residual, h and q stand at the same place in their chunks of 8 elements.
@@ -65,15 +64,10 @@ int launch_row_quant(const RowQuantParams& p, cudaStream_t st) {
     if (chunks <= 4096) return launch_chunks<1024, 4, NORM>(p, gains16, st);
   }
   const unsigned rows = static_cast<unsigned>(p.M);
-  if (p.H <= 256)
-    glp::row_quant_any_kernel<32, 8, NORM><<<(rows + 3) / 4, 128, 0, st>>>(p);
-  else if (p.H <= 2048)
-    glp::row_quant_any_kernel<128, 16, NORM><<<rows, 128, 0, st>>>(p);
-  else if (p.H <= 8192)
-    glp::row_quant_any_kernel<512, 16, NORM><<<rows, 512, 0, st>>>(p);
-  else
-    glp::row_quant_any_kernel<1024, 32, NORM><<<rows, 1024, 0, st>>>(p);
-  return launched();
+  if (p.H <= 256) return launch(glp::row_quant_any_kernel<32, 8, NORM>, (rows + 3) / 4, 128, 0, 1, st, p);
+  if (p.H <= 2048) return launch(glp::row_quant_any_kernel<128, 16, NORM>, rows, 128, 0, 1, st, p);
+  if (p.H <= 8192) return launch(glp::row_quant_any_kernel<512, 16, NORM>, rows, 512, 0, 1, st, p);
+  return launch(glp::row_quant_any_kernel<1024, 32, NORM>, rows, 1024, 0, 1, st, p);
 }
 
 int norm_residual_q8(const glp_norm_q8_args* a, cudaStream_t st) {

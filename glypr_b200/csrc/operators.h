@@ -34,6 +34,27 @@ inline int launched(cudaError_t e = cudaGetLastError()) {
   return e == cudaErrorMemoryAllocation ? GLP_ERR_OOM : GLP_ERR_CUDA;
 }
 
+// One launch, as a programmatic dependent launch: the kernel may start while the one before it in the
+// stream still runs, and waits for that one's end (griddep_wait) before it touches global memory.
+template <class... Params, class... Args>
+int launch(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, int cluster, cudaStream_t st,
+           const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 inline int dtype_size(int dtype) {
   return dtype == GLP_DTYPE_F32 ? 4 : (dtype == GLP_DTYPE_F16 || dtype == GLP_DTYPE_BF16) ? 2 : 1;
 }

@@ -101,6 +101,8 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
   constexpr int ROWS = G < 128 ? 128 / G : 1;
   const int t = threadIdx.x % G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G;
+  griddep_launch();
+  griddep_wait();
   if (row >= p.M) return;  // whole warps or the whole block
   float v[NC];
 #pragma unroll
@@ -341,6 +343,8 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
   constexpr int ROWS = G == 32 ? 8 : 1;
   const int t = threadIdx.x % G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G;
+  griddep_launch();
+  griddep_wait();
   if (row >= p.M) return;  // whole warps or the whole block
   const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * kBytes<XT>;
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
