@@ -25,7 +25,7 @@ struct RowQuantParams {
   void* q;
   float* scale;
   int64_t ld_x, ld_residual, ld_h, ld_q;
-  float eps, layer_scalar;
+  float eps, layer_scalar, inv_H;
   int x_dtype, h_dtype, q_dtype;
 };
 
@@ -63,13 +63,13 @@ __device__ __forceinline__ uint8_t code_of(float v, int q_dtype) {
   return q_dtype == kI8 ? code_i8(v) : static_cast<uint8_t>(code_e4m3x2(v, 0.0f));
 }
 
-// sum of a and NaN-keeping maximum of b over the G threads that share a row (G a warp or the block)
-template <int G>
+// sum of a (SUM) and NaN-keeping maximum of b (MAX) over the G threads that share a row (a warp or the block)
+template <int G, bool SUM = true, bool MAX = true>
 __device__ __forceinline__ void row_reduce(float& a, float& b) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+    if constexpr (SUM) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if constexpr (MAX) b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
   }
   if constexpr (G > 32) {
     __shared__ float2 part[G / 32];
@@ -80,8 +80,8 @@ __device__ __forceinline__ void row_reduce(float& a, float& b) {
     a = part[0].x, b = part[0].y;
 #pragma unroll
     for (int i = 1; i < G / 32; ++i) {
-      a += part[i].x;
-      b = max_nan(b, part[i].y);
+      if constexpr (SUM) a += part[i].x;
+      if constexpr (MAX) b = max_nan(b, part[i].y);
     }
   }
 }
@@ -181,11 +181,11 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no li
 }
 
 // elements [e, e + 8) of the row at `row`, zeros outside [0, H)
-template <int DT>
+template <int DT, bool FULL>
 __device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, int H) {
   constexpr int B = kBytes<DT>;
   Chunk<DT> c;
-  if (e >= 0 && e + 8 <= H) {
+  if (FULL || (e >= 0 && e + 8 <= H)) {
 #pragma unroll
     for (int i = 0; i < B / 2; ++i) c.v[i] = ld_stream(row + static_cast<int64_t>(e) * B + 16 * i);
   } else {
@@ -225,13 +225,13 @@ __device__ __forceinline__ void chunk_f32(const Chunk<DT>& c, uint64_t (&v)[4]) 
   }
 }
 
-template <int DT>
+template <int DT, bool FULL>
 __device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, const uint64_t (&p)[4]) {
   constexpr int B = kBytes<DT>;
   float v[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) f2_split(p[j], v[2 * j], v[2 * j + 1]);
-  if (e >= 0 && e + 8 <= H) {
+  if (FULL || (e >= 0 && e + 8 <= H)) {
     uint8_t* at = row + static_cast<int64_t>(e) * B;
     if constexpr (B == 4) {
       *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
@@ -256,6 +256,7 @@ __device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, const ui
   }
 }
 
+template <bool FULL>
 __device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dtype, const uint64_t (&p)[4], uint64_t k) {
   uint32_t w[2];
   if (q_dtype == kI8) {
@@ -279,7 +280,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dt
     w[0] = __byte_perm(h[0], h[1], 0x5410);
     w[1] = __byte_perm(h[2], h[3], 0x5410);
   }
-  if (e >= 0 && e + 8 <= H) {
+  if (FULL || (e >= 0 && e + 8 <= H)) {
     *reinterpret_cast<uint2*>(row + e) = make_uint2(w[0], w[1]);
   } else {
 #pragma unroll
@@ -301,9 +302,10 @@ __device__ __forceinline__ float max8(float m, const uint64_t (&p)[4]) {
 
 // gain[e .. e + 8) (outside [0, H) any finite value).  e is a multiple of 8 less the row's off: for an
 // unaligned row the aligned words around it are loaded and shifted by off & 3, the same for the whole row.
+template <bool FULL>
 __device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, int H, uint64_t (&p)[4]) {
   const int s = e & 3;
-  if (aligned16 && s == 0 && e >= 0 && e + 8 <= H) {
+  if (FULL || (aligned16 && s == 0 && e >= 0 && e + 8 <= H)) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(gain + e)), b = __ldg(reinterpret_cast<const float4*>(gain + e) + 1);
     p[0] = f2(a.x, a.y), p[1] = f2(a.z, a.w), p[2] = f2(b.x, b.y), p[3] = f2(b.z, b.w);
     return;
@@ -336,9 +338,13 @@ __device__ __forceinline__ float f2_hsum(uint64_t v) {
   return lo + hi;
 }
 
+// rms(v) from the sum of squares
+__device__ __forceinline__ float inv_rms(float ss, const RowQuantParams& p) { return rsqrtf(fmaf(ss, p.inv_H, p.eps)); }
+
 // G threads per row, NC chunks per thread: the row touches at most G NC chunks.  XT, HT: types of x and
-// of residual / h.  gains16: both gains start on 16-byte boundaries.
-template <int G, int NC, int XT, int HT, bool NORM>
+// of residual / h.  gains16: both gains start on 16-byte boundaries.  FULL: every row is exactly G NC whole
+// chunks (and gains16), so no place is checked.
+template <int G, int NC, int XT, int HT, bool NORM, bool FULL>
 __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
   constexpr int ROWS = G == 32 ? 8 : 1;
   const int t = threadIdx.x % G;
@@ -347,10 +353,10 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
   griddep_wait();
   if (row >= p.M) return;  // whole warps or the whole block
   const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * kBytes<XT>;
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
+  const int off = FULL ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
   Chunk<XT> xc[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, (c * G + t) * 8 - off, p.H);
+  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT, FULL>(xr, (c * G + t) * 8 - off, p.H);
   uint8_t* qr = static_cast<uint8_t*>(p.q) + row * p.ld_q;
   uint64_t v[NC][4];
   float none = 0.0f, amax = 0.0f;
@@ -360,21 +366,20 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
     Chunk<HT> rc[NC];
     if (p.residual) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT>(rr, (c * G + t) * 8 - off, p.H);
+      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT, FULL>(rr, (c * G + t) * 8 - off, p.H);
     }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) chunk_f32<XT>(xc[c], v[c]);
     uint64_t inv2 = f2(1.0f, 1.0f);
     if (p.post_gain) {
       uint64_t ss2 = f2(0.0f, 0.0f);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        uint64_t x[4];
-        chunk_f32<XT>(xc[c], x);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ss2 = f2_fma(x[j], x[j], ss2);
-      }
+        for (int j = 0; j < 4; ++j) ss2 = f2_fma(v[c][j], v[c][j], ss2);
       float ss = f2_hsum(ss2);
-      row_reduce<G>(ss, none);
-      const float inv = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+      row_reduce<G, true, false>(ss, none);
+      const float inv = inv_rms(ss, p);
       inv2 = f2(inv, inv);
     }
     const uint64_t scalar2 = f2(p.layer_scalar, p.layer_scalar);
@@ -383,9 +388,8 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
     for (int c = 0; c < NC; ++c) {
       const int e = (c * G + t) * 8 - off;
       uint64_t g[4];
-      chunk_f32<XT>(xc[c], v[c]);
       if (p.post_gain) {
-        load_gain(p.post_gain, gains16, e, p.H, g);
+        load_gain<FULL>(p.post_gain, gains16, e, p.H, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(f2_mul(v[c][j], inv2), g[j]);
       }
@@ -400,34 +404,34 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
         v[c][j] = f2_mul(v[c][j], scalar2);
         ss2 = f2_fma(v[c][j], v[c][j], ss2);
       }
-      if (p.h) store_chunk<HT>(hr, e, p.H, v[c]);
+      if (p.h) store_chunk<HT, FULL>(hr, e, p.H, v[c]);
       if (p.gain) {
-        load_gain(p.gain, gains16, e, p.H, g);
+        load_gain<FULL>(p.gain, gains16, e, p.H, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(v[c][j], g[j]);
       }
       amax = max8(amax, v[c]);
     }
     float ss = f2_hsum(ss2);
-    row_reduce<G>(ss, amax);
-    const float inv_h = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+    row_reduce<G, true, true>(ss, amax);
+    const float inv_h = inv_rms(ss, p);
     const float s = scale_of(amax * inv_h, p.q_dtype);
-    const float k = inv_h / s;
+    const float k = __fdividef(inv_h, s);
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
+    for (int c = 0; c < NC; ++c) store_codes<FULL>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
   } else {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       chunk_f32<XT>(xc[c], v[c]);
       amax = max8(amax, v[c]);
     }
-    row_reduce<G>(none, amax);
+    row_reduce<G, false, true>(none, amax);
     const float s = scale_of(amax, p.q_dtype);
     const float k = 1.0f / s;
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
+    for (int c = 0; c < NC; ++c) store_codes<FULL>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
   }
 }
 
