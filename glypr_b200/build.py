@@ -12,9 +12,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libglypr_cuda.so")
-SOURCES = ["glypr_cuda.cu", "op_rows.cu", "op_linear.cu", "gguf.cpp", "engine.cpp", "tokenizer.cpp"]
+SOURCES = ["glypr_cuda.cu", "op_rows_f32.cu", "op_rows_f16.cu", "op_rows_bf16.cu", "op_rows.cu", "op_linear.cu",
+           "gguf.cpp", "engine.cpp", "tokenizer.cpp"]
 HEADERS = ["common.cuh", "gemm.cuh", "q8gemm.cuh", "attention_tc.cuh", "attention_d512.cuh", "attention_pair.cuh", "rowops.cuh", "gguf.h", "ple.cuh",
-           "rowquant.cuh", "linear.cuh", "linear_any.cuh",
+           "rowquant.cuh", "op_rows.cuh", "linear.cuh", "linear_any.cuh",
            "linear_rows.cuh", "linear_tc.cuh", "operators.h", "unicode_case.inc"]
 
 

@@ -1,9 +1,6 @@
 // Host side of glp_norm_residual_q8 and glp_quantize_rows: argument checks, the choice of kernel,
 // launches.
-#include <type_traits>
-
-#include "operators.h"
-#include "rowquant.cuh"
+#include "op_rows.cuh"
 
 namespace {
 
@@ -12,27 +9,6 @@ using glp::RowQuantParams;
 
 static_assert(GLP_DTYPE_F32 == glp::kF32 && GLP_DTYPE_F16 == glp::kF16 && GLP_DTYPE_BF16 == glp::kBF16 &&
               GLP_DTYPE_I8 == glp::kI8 && GLP_DTYPE_E4M3 == glp::kE4M3, "dtype codes");
-
-template <int G, int NC, bool NORM, bool FULL>
-int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
-  constexpr int ROWS = G == 32 ? 8 : 1;
-  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.M) + ROWS - 1) / ROWS), block = G == 32 ? 256 : G;
-  if constexpr (NORM) {
-    const auto with_h = [&](auto xt) -> int {
-      constexpr int XT = decltype(xt)::value;
-      if (p.h_dtype == GLP_DTYPE_F32) return launch(glp::row_quant_kernel<G, NC, XT, glp::kF32, true, FULL>, grid, block, 0, 1, st, p, gains16);
-      if (p.h_dtype == GLP_DTYPE_F16) return launch(glp::row_quant_kernel<G, NC, XT, glp::kF16, true, FULL>, grid, block, 0, 1, st, p, gains16);
-      return launch(glp::row_quant_kernel<G, NC, XT, glp::kBF16, true, FULL>, grid, block, 0, 1, st, p, gains16);
-    };
-    if (p.x_dtype == GLP_DTYPE_F32) return with_h(std::integral_constant<int, glp::kF32>{});
-    if (p.x_dtype == GLP_DTYPE_F16) return with_h(std::integral_constant<int, glp::kF16>{});
-    return with_h(std::integral_constant<int, glp::kBF16>{});
-  } else {
-    if (p.x_dtype == GLP_DTYPE_F32) return launch(glp::row_quant_kernel<G, NC, glp::kF32, glp::kF32, false, FULL>, grid, block, 0, 1, st, p, false);
-    if (p.x_dtype == GLP_DTYPE_F16) return launch(glp::row_quant_kernel<G, NC, glp::kF16, glp::kF16, false, FULL>, grid, block, 0, 1, st, p, false);
-    return launch(glp::row_quant_kernel<G, NC, glp::kBF16, glp::kBF16, false, FULL>, grid, block, 0, 1, st, p, false);
-  }
-}
 
 // Whether every row's x, residual, h and q stand at the same place in their chunks of 8 elements.
 bool same_chunks(const RowQuantParams& p) {
@@ -46,29 +22,18 @@ bool same_chunks(const RowQuantParams& p) {
 
 template <bool NORM>
 int launch_row_quant(const RowQuantParams& p, cudaStream_t st) {
-  if (same_chunks(p)) {
-    const bool gains16 = aligned(p.gain, 16) && aligned(p.post_gain, 16);
-    // a row that starts inside a chunk touches one more
-    const int dx = dtype_size(p.x_dtype);
-    const bool flush = reinterpret_cast<uintptr_t>(p.x) / dx % 8 == 0 && p.ld_x % 8 == 0;
-    const int chunks = (p.H + (flush ? 7 : 14)) / 8;
-    const bool full = flush && p.H % 8 == 0 && (gains16 || !NORM);
-    if (full && chunks == 32) return launch_chunks<32, 1, NORM, true>(p, gains16, st);
-    if (full && chunks == 64) return launch_chunks<32, 2, NORM, true>(p, gains16, st);
-    if (full && chunks == 96) return launch_chunks<32, 3, NORM, true>(p, gains16, st);
-    if (full && chunks == 128) return launch_chunks<32, 4, NORM, true>(p, gains16, st);
-    if (full && chunks == 256) return launch_chunks<128, 2, NORM, true>(p, gains16, st);
-    if (full && chunks == 512) return launch_chunks<128, 4, NORM, true>(p, gains16, st);
-    if (chunks <= 32) return launch_chunks<32, 1, NORM, false>(p, gains16, st);
-    if (chunks <= 64) return launch_chunks<32, 2, NORM, false>(p, gains16, st);
-    if (chunks <= 96) return launch_chunks<32, 3, NORM, false>(p, gains16, st);
-    if (chunks <= 128) return launch_chunks<32, 4, NORM, false>(p, gains16, st);
-    if (chunks <= 160) return launch_chunks<32, 5, NORM, false>(p, gains16, st);
-    if (chunks <= 256) return launch_chunks<128, 2, NORM, false>(p, gains16, st);
-    if (chunks <= 512) return launch_chunks<128, 4, NORM, false>(p, gains16, st);
-    if (chunks <= 1024) return launch_chunks<512, 2, NORM, false>(p, gains16, st);
-    if (chunks <= 2048) return launch_chunks<512, 4, NORM, false>(p, gains16, st);
-    if (chunks <= 4096) return launch_chunks<1024, 4, NORM, false>(p, gains16, st);
+  const bool at_chunk = reinterpret_cast<uintptr_t>(p.x) / dtype_size(p.x_dtype) % 8 == 0 && p.ld_x % 8 == 0;
+  if (same_chunks(p) && (at_chunk || (p.H + 14) / 8 <= GLP_QUANT_MAX_H / 8)) {  // (else one chunk too many)
+    if constexpr (NORM) {
+      const bool gains16 = aligned(p.gain, 16) && aligned(p.post_gain, 16);
+      if (p.x_dtype == GLP_DTYPE_F32) return launch_norm_chunks<glp::kF32>(p, gains16, st);
+      if (p.x_dtype == GLP_DTYPE_F16) return launch_norm_chunks<glp::kF16>(p, gains16, st);
+      return launch_norm_chunks<glp::kBF16>(p, gains16, st);
+    } else {
+      if (p.x_dtype == GLP_DTYPE_F32) return launch_quant_chunks<glp::kF32>(p, st);
+      if (p.x_dtype == GLP_DTYPE_F16) return launch_quant_chunks<glp::kF16>(p, st);
+      return launch_quant_chunks<glp::kBF16>(p, st);
+    }
   }
   const unsigned rows = static_cast<unsigned>(p.M);
   if (p.H <= 256) return launch(glp::row_quant_any_kernel<32, 8, NORM>, (rows + 3) / 4, 128, 0, 1, st, p);

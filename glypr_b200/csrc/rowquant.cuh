@@ -166,6 +166,14 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
 // one 8-byte store of codes).  Rows need not start on a chunk boundary -- a packed odd width has no two
 // rows alike -- as long as x, residual, h and q all stand at the same place in their chunks: chunk i of
 // a row is elements [8 i - off, 8 i - off + 8), and only the two at the row's ends go by element.
+// how a row lies in its chunks: anywhere; from a chunk's start, in whole chunks; and exactly as many as
+// its threads hold
+constexpr int kShifted = 0, kFlush = 1, kFull = 2;
+template <int PLACE>
+__device__ __forceinline__ bool whole_chunk(int e, int H) {
+  return PLACE == kFull || (PLACE == kFlush ? e < H : e >= 0 && e + 8 <= H);
+}
+
 template <int DT>
 constexpr int kBytes = DT == kF32 ? 4 : 2;
 
@@ -181,11 +189,11 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no li
 }
 
 // elements [e, e + 8) of the row at `row`, zeros outside [0, H)
-template <int DT, bool FULL>
+template <int DT, int PLACE>
 __device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, int H) {
   constexpr int B = kBytes<DT>;
   Chunk<DT> c;
-  if (FULL || (e >= 0 && e + 8 <= H)) {
+  if (whole_chunk<PLACE>(e, H)) {
 #pragma unroll
     for (int i = 0; i < B / 2; ++i) c.v[i] = ld_stream(row + static_cast<int64_t>(e) * B + 16 * i);
   } else {
@@ -195,7 +203,7 @@ __device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, int H
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int n = e + j;
-      if (n >= 0 && n < H) {
+      if (PLACE == kShifted && n >= 0 && n < H) {
         if constexpr (B == 4)
           w[j] = *reinterpret_cast<const uint32_t*>(row + static_cast<int64_t>(n) * 4);
         else
@@ -225,13 +233,13 @@ __device__ __forceinline__ void chunk_f32(const Chunk<DT>& c, uint64_t (&v)[4]) 
   }
 }
 
-template <int DT, bool FULL>
+template <int DT, int PLACE>
 __device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, const uint64_t (&p)[4]) {
   constexpr int B = kBytes<DT>;
   float v[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) f2_split(p[j], v[2 * j], v[2 * j + 1]);
-  if (FULL || (e >= 0 && e + 8 <= H)) {
+  if (whole_chunk<PLACE>(e, H)) {
     uint8_t* at = row + static_cast<int64_t>(e) * B;
     if constexpr (B == 4) {
       *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
@@ -249,14 +257,14 @@ __device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, const ui
       }
       *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-  } else {
+  } else if (PLACE == kShifted) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (e + j >= 0 && e + j < H) store_from_f32(row, e + j, DT, v[j]);
   }
 }
 
-template <bool FULL>
+template <int PLACE>
 __device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dtype, const uint64_t (&p)[4], uint64_t k) {
   uint32_t w[2];
   if (q_dtype == kI8) {
@@ -280,9 +288,9 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dt
     w[0] = __byte_perm(h[0], h[1], 0x5410);
     w[1] = __byte_perm(h[2], h[3], 0x5410);
   }
-  if (FULL || (e >= 0 && e + 8 <= H)) {
+  if (whole_chunk<PLACE>(e, H)) {
     *reinterpret_cast<uint2*>(row + e) = make_uint2(w[0], w[1]);
-  } else {
+  } else if (PLACE == kShifted) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (e + j >= 0 && e + j < H) row[e + j] = static_cast<uint8_t>(w[j / 4] >> (8 * (j & 3)));
@@ -302,10 +310,14 @@ __device__ __forceinline__ float max8(float m, const uint64_t (&p)[4]) {
 
 // gain[e .. e + 8) (outside [0, H) any finite value).  e is a multiple of 8 less the row's off: for an
 // unaligned row the aligned words around it are loaded and shifted by off & 3, the same for the whole row.
-template <bool FULL>
+template <int PLACE>
 __device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, int H, uint64_t (&p)[4]) {
+  if (PLACE != kShifted && e >= H) {  // (only where the chunk is empty: its values are zeros)
+    p[0] = p[1] = p[2] = p[3] = f2(0.0f, 0.0f);
+    return;
+  }
   const int s = e & 3;
-  if (FULL || (aligned16 && s == 0 && e >= 0 && e + 8 <= H)) {
+  if (PLACE != kShifted || (aligned16 && s == 0 && e >= 0 && e + 8 <= H)) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(gain + e)), b = __ldg(reinterpret_cast<const float4*>(gain + e) + 1);
     p[0] = f2(a.x, a.y), p[1] = f2(a.z, a.w), p[2] = f2(b.x, b.y), p[3] = f2(b.z, b.w);
     return;
@@ -342,9 +354,9 @@ __device__ __forceinline__ float f2_hsum(uint64_t v) {
 __device__ __forceinline__ float inv_rms(float ss, const RowQuantParams& p) { return rsqrtf(fmaf(ss, p.inv_H, p.eps)); }
 
 // G threads per row, NC chunks per thread: the row touches at most G NC chunks.  XT, HT: types of x and
-// of residual / h.  gains16: both gains start on 16-byte boundaries.  FULL: every row is exactly G NC whole
-// chunks (and gains16), so no place is checked.
-template <int G, int NC, int XT, int HT, bool NORM, bool FULL>
+// of residual / h.  gains16: both gains start on 16-byte boundaries.  PLACE
+// kFlush and kFull also promise gains16.
+template <int G, int NC, int XT, int HT, bool NORM, int PLACE>
 __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
   constexpr int ROWS = G == 32 ? 8 : 1;
   const int t = threadIdx.x % G;
@@ -353,10 +365,10 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
   griddep_wait();
   if (row >= p.M) return;  // whole warps or the whole block
   const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * kBytes<XT>;
-  const int off = FULL ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
+  const int off = PLACE != kShifted ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
   Chunk<XT> xc[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT, FULL>(xr, (c * G + t) * 8 - off, p.H);
+  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT, PLACE>(xr, (c * G + t) * 8 - off, p.H);
   uint8_t* qr = static_cast<uint8_t*>(p.q) + row * p.ld_q;
   uint64_t v[NC][4];
   float none = 0.0f, amax = 0.0f;
@@ -366,7 +378,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
     Chunk<HT> rc[NC];
     if (p.residual) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT, FULL>(rr, (c * G + t) * 8 - off, p.H);
+      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT, PLACE>(rr, (c * G + t) * 8 - off, p.H);
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) chunk_f32<XT>(xc[c], v[c]);
@@ -389,7 +401,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
       const int e = (c * G + t) * 8 - off;
       uint64_t g[4];
       if (p.post_gain) {
-        load_gain<FULL>(p.post_gain, gains16, e, p.H, g);
+        load_gain<PLACE>(p.post_gain, gains16, e, p.H, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(f2_mul(v[c][j], inv2), g[j]);
       }
@@ -404,9 +416,9 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
         v[c][j] = f2_mul(v[c][j], scalar2);
         ss2 = f2_fma(v[c][j], v[c][j], ss2);
       }
-      if (p.h) store_chunk<HT, FULL>(hr, e, p.H, v[c]);
+      if (p.h) store_chunk<HT, PLACE>(hr, e, p.H, v[c]);
       if (p.gain) {
-        load_gain<FULL>(p.gain, gains16, e, p.H, g);
+        load_gain<PLACE>(p.gain, gains16, e, p.H, g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(v[c][j], g[j]);
       }
@@ -419,7 +431,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
     const float k = __fdividef(inv_h, s);
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes<FULL>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
+    for (int c = 0; c < NC; ++c) store_codes<PLACE>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
   } else {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -431,7 +443,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
     const float k = 1.0f / s;
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes<FULL>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
+    for (int c = 0; c < NC; ++c) store_codes<PLACE>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
   }
 }
 
