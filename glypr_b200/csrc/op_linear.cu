@@ -184,6 +184,8 @@ bool tc_operands(const LinearParams& p) {
 int linear(const glp_linear_args* a, cudaStream_t st) {
   if (!a) return fail(GLP_ERR_INVALID_ARG, "args is NULL");
   if (a->M < 0 || a->N < 1 || a->K < 1) return fail(GLP_ERR_INVALID_ARG, "linear needs M >= 0, N >= 1, K >= 1");
+  if (a->M > 1 << 30 || a->N > 1 << 30 || a->K > 1 << 28)  // indices of rows and bytes of a row stay in 31 bits
+    return fail(GLP_ERR_INVALID_ARG, "linear needs M and N <= 2^30, K <= 2^28");
   if (a->dtype < GLP_DTYPE_F16 || a->dtype > GLP_DTYPE_E4M3)
     return fail(GLP_ERR_INVALID_ARG, "operands must be F16, BF16, I8 or E4M3");
   if (!wide_dtype(a->out_dtype)) return fail(GLP_ERR_INVALID_ARG, "y must be F32, F16 or BF16");

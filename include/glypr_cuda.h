@@ -417,7 +417,9 @@ typedef struct glp_linear_args {
 /* y = act(x w^T * x_scale * w_scale + bias) [* (x w_up^T * x_scale * w_up_scale + bias_up)] + residual
  * with products summed in f32 (I8: exactly, in int32; K <= 131071) and one rounding to out_dtype.
  * Rows of x, w and w_up that start on 16-byte boundaries (base addresses and pitches) run on the
- * tensor cores; any other alignment is accepted and slower. */
+ * tensor cores; any other alignment is accepted and slower (so are rows of y or residual off
+ * 16-byte boundaries, by less).  M and N up to 2^30, K up to 2^28.  Which kernel runs goes by the
+ * sizes, so a row's value may differ in the last bits between batches of another M. */
 int glp_linear(const glp_linear_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -99,7 +99,8 @@ def run_quantize(x, q, scale, xd, qd, stream=0):
                       ld_q=q.stride(0), stream=stream)
 
 
-@pytest.mark.parametrize("h", [1, 7, 64, 255, 256, 768, 1152, 1543, 2056, 4096, 8200, 20000, 32768])
+@pytest.mark.parametrize("h", [1, 7, 64, 255, 256, 512, 768, 1152, 1500, 1543, 1790, 2056, 3000, 4096, 5000, 6101, 8000,
+                               8200, 12000, 20000, 32761, 32768])
 @pytest.mark.parametrize("xd,qd", [("f16", "i8"), ("bf16", "e4m3"), ("f32", "i8"), ("f32", "e4m3")])
 def test_quantize_rows(h, xd, qd):
     for m, pad, off in ((1, 0, 0), (5, 0, 0), (67, 8, 8), (33, 3, 1)):
@@ -161,7 +162,8 @@ def norm_want(x, res, post, gain, scalar):
                              .clamp_min(1e-300)) * (1 if gain is None else gain.abs())
 
 
-@pytest.mark.parametrize("h", [1, 5, 64, 256, 768, 1024, 1152, 1543, 2048, 2568, 4096, 9001, 16384, 32768])
+@pytest.mark.parametrize("h", [1, 5, 64, 256, 512, 768, 1024, 1152, 1543, 2048, 2568, 4096, 5000, 6000, 8000, 9001,
+                               12000, 16384, 20004, 32761, 32768])
 @pytest.mark.parametrize("xd,hd,qd", [("f16", "bf16", "i8"), ("bf16", "bf16", "e4m3"), ("f32", "f32", "i8"),
                                       ("f16", "f32", "e4m3"), ("f32", "f16", "e4m3")])
 def test_norm_residual_q8(h, xd, hd, qd):
@@ -191,8 +193,9 @@ def test_norm_residual_q8(h, xd, hd, qd):
         check_codes(q, scale, n_want, qd, n_mag)
 
 
-def test_norm_in_place_and_without_h():
-    m, h = 37, 768
+@pytest.mark.parametrize("h", [768, 771, 2048, 2051, 9001])
+def test_norm_in_place_and_without_h(h):
+    m = 37
     x, res = filled(rows_of(m, h, 1), "f16"), filled(rows_of(m, h, 2), "bf16")
     gain = rows_of(1, h, 3, 0.0)[0] * 0.1 + 1
     outs = []
@@ -340,6 +343,31 @@ def test_linear_sizes(m, n, k, dtype, out):
     c = Case(m, n, k, dtype, out, act="silu", gated=True, bias=True, res=(m % 2 == 1), seed=m + n + k + 9)
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 2500, 300), (16, 2376, 72), (20, 2400, 80), (32, 1300, 200), (40, 2400, 100),
+                                   (64, 96, 1000), (33, 4100, 1040), (20, 7300, 700)])
+@pytest.mark.parametrize("dtype,out", [("f16", "f32"), ("bf16", "f16"), ("i8", "f32"), ("e4m3", "bf16")])
+def test_linear_few_rows_of_many_columns(m, n, k, dtype, out):
+    """Either side of the rules that choose how many rows of w a block of the few-rows kernel takes, and
+    between it and the tensor-memory kernel."""
+    for gated in (False, True):
+        c = Case(m, n, k, dtype, out, act="gelu_erf", gated=gated, bias=True, res=True, seed=m + n)
+        c.run()
+        c.check()
+
+
+@pytest.mark.parametrize("dtype,k", [("f16", 1000), ("bf16", 1056), ("i8", 2100), ("e4m3", 2064)])
+@pytest.mark.parametrize("n,ypad,yoff", [(520, 0, 0), (777, 0, 0), (777, 7, 0), (520, 3, 5), (264, 8, 8)])
+def test_linear_on_pairs(dtype, k, n, ypad, yoff):
+    """Products of enough 256 x 256 tiles for the CTA-pair kernel: several tiles per pair, ragged last
+    tiles, outputs on and off 16-byte rows, each epilogue's warps."""
+    for m, act, gated, res, out in ((20011, "none", False, True, "bf16"), (20011, "gelu_erf", False, True, "f16"),
+                                    (16384, "silu", True, True, "f16"), (20011, "relu", False, True, "f32"),
+                                    (19999, "gelu_tanh", True, False, "f32"), (16385, "none", False, False, "f16")):
+        c = Case(m, n, k, dtype, out, act=act, gated=gated, bias=True, res=res, seed=n + k, ypad=ypad, yoff=yoff)
+        c.run()
+        c.check()
 
 
 @pytest.mark.parametrize("m,n,k", [(4, 200, 320), (70, 200, 320), (700, 520, 192)])

@@ -27,7 +27,8 @@ def linear(m=4, n=8, k=16, dtype="f16", x=P, w=P, y=P, out="f16", **kw):
     (linear(dtype="f32"), "operands"), (linear(dtype=9), "operands"), (linear(dtype=-1), "operands"),
     (linear(out="i8"), "y must be"), (linear(out="e4m3"), "y must be"), (linear(out=7), "y must be"),
     (linear(activation=5), "activation"), (linear(activation=-1), "activation"),
-    (linear(dtype="i8", k=131072), "131071"),
+    (linear(dtype="i8", k=131072), "131071"), (linear(m=2 ** 30 + 1), "2^30"), (linear(n=2 ** 30 + 1), "2^30"),
+    (linear(k=2 ** 28 + 1), "2^28"),
     (linear(x=0), "null"), (linear(w=0), "null"), (linear(y=0), "null"),
     (linear(ldx=15), "shorter than K"), (linear(ldw=15), "shorter than K"), (linear(ldx=-16), "shorter than K"),
     (linear(ldy=7), "shorter than N"), (linear(residual=P, ld_residual=7), "shorter than N"),
