@@ -8,6 +8,8 @@
 //!   beside `MetalQ8_0` (linear.rs:6-15, forward at linear.rs:150-172) over device pointers.
 //! * [`flash_attention`] -- the `AttentionMode::CudaFlash` slot (attention/mod.rs:255-262,
 //!   `AttentionBackend::compute_attention`, attention/traits.rs:37-46).
+//! * [`norm_residual_q8`], [`quantize_rows`], [`linear`] -- 8-bit activations with a scale per row, and the
+//!   matrix product with bias, activation, gate and residual over 8-bit or 16-bit operands.
 //! * [`Engine`] -- the server's batching worker (glypr-server/src/engine.rs:157-325).
 //! * [`Tokenizer`] -- `GlyprTokenizer::from_gguf_metadata` / `encode` (tokenizer.rs:77-229).
 //!
@@ -185,6 +187,41 @@ impl CudaQ8Linear {
             stream,
         ))
     }
+}
+
+/// Residual addition and RMS norm with the output in 8 bits (`glp_norm_residual_q8`).
+///
+/// # Safety
+/// The pointers of `args` are device pointers on the current CUDA device, sized as the header says.
+pub unsafe fn norm_residual_q8(args: &ffi::glp_norm_q8_args, stream: *mut c_void) -> Result<()> {
+    check(ffi::glp_norm_residual_q8(args, stream))
+}
+
+/// The 8-bit form of `m` packed rows of `h` elements (`glp_quantize_rows`): codes and one scale per row.
+///
+/// # Safety
+/// `x`, `q` and `scale` are device pointers on the current CUDA device to `m * h` elements of `x_dtype`,
+/// `m * h` codes and `m` f32.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn quantize_rows(
+    x: *const c_void,
+    x_dtype: i32,
+    m: usize,
+    h: usize,
+    q: *mut c_void,
+    q_dtype: i32,
+    scale: *mut f32,
+    stream: *mut c_void,
+) -> Result<()> {
+    check(ffi::glp_quantize_rows(x, x_dtype, 0, m as c_int, h as c_int, q, q_dtype, 0, scale, stream))
+}
+
+/// `y = act(x w^T * scales + bias) [* (x w_up^T * scales + bias_up)] + residual` (`glp_linear`).
+///
+/// # Safety
+/// The pointers of `args` are device pointers on the current CUDA device, sized as the header says.
+pub unsafe fn linear(args: &ffi::glp_linear_args, stream: *mut c_void) -> Result<()> {
+    check(ffi::glp_linear(args, stream))
 }
 
 /// `AttentionMode::CudaFlash` over a packed, normed and RoPE'd qkv tensor

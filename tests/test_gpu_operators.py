@@ -532,3 +532,15 @@ def test_operators_together():
     # noise per value, under 1.2 % of the row's rms for maxima of up to 5 rms; five of them
     # (three weights, two activations; gate and up both enter a) stay under 4 % in the 2-norm
     assert float((y.double() - y64).norm() / y64.norm()) < 0.04
+
+
+def test_the_example_runs():
+    """examples/int8_feed_forward.py end to end: the same noise bound as above."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "int8_feed_forward.py")
+    spec = importlib.util.spec_from_file_location("int8_feed_forward", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    err, cos = example.main(["--tokens", "333"])
+    assert err < 0.04 and cos > 0.998
