@@ -16,7 +16,7 @@ SOURCES = ["glypr_cuda.cu", "op_rows_f32.cu", "op_rows_f16.cu", "op_rows_bf16.cu
            "gguf.cpp", "engine.cpp", "tokenizer.cpp"]
 HEADERS = ["common.cuh", "gemm.cuh", "q8gemm.cuh", "attention_tc.cuh", "attention_d512.cuh", "attention_pair.cuh", "rowops.cuh", "gguf.h", "ple.cuh",
            "rowquant.cuh", "op_rows.cuh", "linear.cuh", "linear_any.cuh",
-           "linear_rows.cuh", "linear_tc.cuh", "operators.h", "unicode_case.inc"]
+           "linear_rows.cuh", "linear_tc.cuh", "linear_splitk.cuh", "operators.h", "unicode_case.inc"]
 
 
 def nvcc() -> str:

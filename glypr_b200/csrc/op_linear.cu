@@ -4,6 +4,7 @@
 
 #include "linear_any.cuh"
 #include "linear_rows.cuh"
+#include "linear_splitk.cuh"
 #include "linear_tc.cuh"
 #include "operators.h"
 
@@ -71,17 +72,23 @@ uint32_t mma_idesc(int dtype, int m, int n) {
   return acc << 4 | ab << 7 | ab << 10 | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
 }
 
+// raises a kernel's shared-memory limit once per device
+template <class K>
+int raise_smem(K kernel, size_t smem, int dev, std::atomic<uint64_t>* ready) {
+  const uint64_t bit = 1ull << dev;
+  if (ready->load(std::memory_order_relaxed) & bit) return GLP_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return fail(GLP_ERR_CUDA, cudaGetErrorString(e));
+  ready->fetch_or(bit, std::memory_order_relaxed);
+  return GLP_OK;
+}
+
 template <int KIND, int CG, int BN, bool GATED, int EPI = 8>
 int launch_tc(glp::LinearTcParams p, const DeviceInfo& d, cudaStream_t st) {
   using Cfg = glp::LinearTcCfg<CG, BN, GATED, EPI>;
   const auto kernel = glp::linear_tc_kernel<KIND, CG, BN, GATED, EPI>;
-  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
-  const uint64_t bit = 1ull << d.dev;
-  if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::SMEM));
-    if (e != cudaSuccess) return fail(GLP_ERR_CUDA, cudaGetErrorString(e));
-    ready.fetch_or(bit, std::memory_order_relaxed);
-  }
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = raise_smem(kernel, Cfg::SMEM, d.dev, &ready)) return rc;
   const LinearParams& a = p.a;
   p.m_tiles = (a.M + 128 * CG - 1) / (128 * CG);
   p.n_tiles = (a.N + Cfg::OUT_N - 1) / Cfg::OUT_N;
@@ -109,24 +116,65 @@ int launch_tc(glp::LinearTcParams p, const DeviceInfo& d, cudaStream_t st) {
   return launch(kernel, static_cast<unsigned>(units * CG), Cfg::THREADS, Cfg::SMEM, CG, st, mx, mw, mu, mr, my, p);
 }
 
+template <int KIND, bool GATED, int S>
+int launch_split(glp::LinearTcParams p, const DeviceInfo& d, cudaStream_t st) {
+  using Cfg = glp::LinearSplitCfg<GATED>;
+  const auto kernel = glp::linear_split_kernel<KIND, GATED, S>;
+  static std::atomic<uint64_t> ready{0};
+  if (int rc = raise_smem(kernel, Cfg::SMEM, d.dev, &ready)) return rc;
+  const LinearParams& a = p.a;
+  p.m_tiles = (a.M + 127) / 128;
+  p.n_tiles = (a.N + 63) / 64;
+  p.k_step = 128 / dtype_size(a.dtype);
+  p.k_blocks = (a.K + p.k_step - 1) / p.k_step;
+  p.idesc = mma_idesc(a.dtype, 128, Cfg::BN);
+  CUtensorMap mx, mw, mu;
+  if (int rc = make_map(&mx, a.x, a.dtype, a.M, a.K, a.ld_x, 128)) return rc;
+  if (int rc = make_map(&mw, a.w, a.dtype, a.N, a.K, a.ld_w, 64)) return rc;
+  mu = mw;
+  if (GATED)
+    if (int rc = make_map(&mu, a.w_up, a.dtype, a.N, a.K, a.ld_w, 64)) return rc;
+  return launch(kernel, static_cast<unsigned>(p.m_tiles * p.n_tiles * S), Cfg::THREADS, Cfg::SMEM, S, st, mx, mw, mu, p);
+}
+
 template <int KIND>
 int launch_tc_kind(const LinearParams& a, const DeviceInfo& d, cudaStream_t st) {
   glp::LinearTcParams p{};
   p.a = a;
   p.a.status = d.status;
   const bool gated = a.w_up != nullptr;
-  // The tile by estimated time: a fixed part, and per wave of tiles the K steps (128 bytes of a row each)
-  // or, with few of them, the drain.  Microseconds, read off M = 512 .. 16,384 against N x K of 768 x 768
-  // f16, 768 x 1,152 and 2,304 x 768 int8, 4,096 x 4,096 e4m3 with bias and residual, and gated 1,152 x 768
-  // int8; e.g. M = 512, 768 x 768 f16: 64-wide 7.3, 128-wide 8.2, pairs 11.1; M = 4,096: 15.1, 12.9, 11.9.
+  // The kernel by estimated time: a fixed part, and per wave of tiles the K steps (128 bytes of a row each)
+  // or, with few of them, the drain.  Microseconds in a CUDA graph, read off M = 65 .. 16,384 against N x K of
+  // 768 x 768 f16, 768 x 1,152 and 2,304 x 768 int8, 4,096 x 4,096 e4m3, 2,048 x 2,048 bf16 and 300 x 8,000 f16
+  // with bias and residual, and gated 1,152 x 768 int8 and x 4,096 bf16.  768 x 768 f16: M = 512: 64-wide 6.5,
+  // 128-wide 8.2, pairs 11; M = 4,096: 15, 12.9, 12.  Splitting K over clusters of 2, 4, 8 (one wave of them,
+  // fewer than SMs since a cluster stays within a GPC): 300 x 8,000 f16, M = 128: 37.6 unsplit, 22.3, 13.0,
+  // 9.0; 4,096 x 4,096 e4m3, M = 128: 12.1, 9.7 with 2.
   const int steps = (a.K * dtype_size(a.dtype) + 127) / 128;
   const auto estimate = [&](int64_t rows, int64_t cols, int64_t slots, double fixed, double step, double drain) {
     const int64_t tiles = ((a.M + rows - 1) / rows) * ((a.N + cols - 1) / cols);
     return fixed + static_cast<double>((tiles + slots - 1) / slots) * std::max(step * steps, drain);
   };
   const double pair = estimate(256, gated ? 128 : 256, d.sms / 2, 5.0, 0.43, gated ? 3.5 : 5.4);
-  const double single128 = estimate(128, gated ? 64 : 128, d.sms, 3.5, 0.37, gated ? 2.5 : 3.15);
-  const double single64 = gated ? 1e30 : estimate(128, 64, d.sms, 3.6, 0.31, 2.0);
+  const double single128 = estimate(128, gated ? 64 : 128, d.sms, 3.2, 0.37, gated ? 2.5 : 3.15);
+  const double single64 = gated ? 1e30 : estimate(128, 64, d.sms, 2.9, 0.29, 2.0);
+  const int64_t tiles64 = ((a.M + 127ll) / 128) * ((a.N + 63ll) / 64);
+  int split = 1;
+  double best = std::min({pair, single128, single64});
+  for (const int S : {2, 4, 8}) {
+    const int64_t room = S == 2 ? d.sms : S == 4 ? d.sms * 7 / 8 : d.sms * 3 / 4;
+    const double t = (gated ? 6.8 : 4.6) + (S == 8 ? 0.4 : 0.0) + 0.285 * ((steps + S - 1) / S);
+    if (tiles64 * S <= room && steps >= 2 * S && t < best) {
+      best = t;
+      split = S;
+    }
+  }
+  switch (split) {
+    case 2: return gated ? launch_split<KIND, true, 2>(p, d, st) : launch_split<KIND, false, 2>(p, d, st);
+    case 4: return gated ? launch_split<KIND, true, 4>(p, d, st) : launch_split<KIND, false, 4>(p, d, st);
+    case 8: return gated ? launch_split<KIND, true, 8>(p, d, st) : launch_split<KIND, false, 8>(p, d, st);
+    default: break;
+  }
   if (pair <= single128 && pair <= single64) {
     // 16 warps drain a tile whose outputs take two exponentials or reciprocals each: their phases (tensor
     // memory, special functions, stores) then overlap between warps.  131,072 x 2,304 x 768 e4m3 with SiLU:

@@ -357,6 +357,21 @@ def test_linear_few_rows_of_many_columns(m, n, k, dtype, out):
         c.check()
 
 
+@pytest.mark.parametrize("m,n,k", [(100, 300, 3000), (65, 2049, 2100), (128, 64, 8100), (257, 777, 1600), (130, 61, 2056),
+                                   (500, 520, 2064)])
+@pytest.mark.parametrize("dtype,out", [("f16", "f16"), ("bf16", "f32"), ("i8", "f32"), ("e4m3", "bf16")])
+def test_linear_split_over_k(m, n, k, dtype, out):
+    """Few tiles and a long K: clusters of 2, 4 and 8 CTAs share a tile's K steps."""
+    for act, gated, bias, res in (("none", False, False, False), ("gelu_tanh", False, True, True), ("silu", True, True, True)):
+        c = Case(m, n, k, dtype, out, act=act, gated=gated, bias=bias, res=res, seed=m + k, ypad=(3 if gated else 0))
+        c.run()
+        c.check()
+        again = torch.empty_like(c.y)
+        again.copy_(c.y)
+        c.run()
+        assert torch.equal(again, c.y)
+
+
 @pytest.mark.parametrize("dtype,k", [("f16", 1000), ("bf16", 1056), ("i8", 2100), ("e4m3", 2064)])
 @pytest.mark.parametrize("n,ypad,yoff", [(520, 0, 0), (777, 0, 0), (777, 7, 0), (520, 3, 5), (264, 8, 8)])
 def test_linear_on_pairs(dtype, k, n, ypad, yoff):
