@@ -4,6 +4,10 @@
 // cluster owns columns [r 64/S, (r + 1) 64/S): every CTA stores its partial sums of those columns into
 // r's shared memory, and after one cluster barrier r adds the S of them in rank order (int8: exactly, in
 // int32), applies the epilogue and writes its columns.  Nothing is left in global memory between calls.
+// What its columns need besides the sums is fetched before the products end: fetched after the barrier it
+// cost 3 us more (768 x 768 f16, M = 128, S = 2: 9.3 us, 6.3 us).  The time is latency: 0.285 us per K step of
+// a CTA on 4.6 us (gated 6.8 us) for launch, first load, exchange and stores.  300 x 8,000 f16, M = 128: 9.0 us
+// with S = 8, 37.6 us unsplit (the plain bytes: 1.1 us).
 #pragma once
 #include "linear_tc.cuh"
 

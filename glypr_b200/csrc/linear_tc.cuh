@@ -17,7 +17,21 @@
 // The residual rows come by TMA into the same 32-row x 128-byte boxes that the outputs leave from,
 // and y may be the residual itself: a box is read before the same box is stored, and no other warp
 // touches its elements.  Where y or residual does not suit TMA (16-byte base and pitch) the box holds
-// 32 f32 columns and the warp writes them out row by row, one element per lane.
+// 32 f32 columns and the warp writes them out row by row, one element per lane (26,943 x 4,055 x 161 int8
+// with residual: 197 us, 130 us with 4,056 columns).
+//
+// What bounds it, on a B200 at its 1 kW limit: the large products draw it and run at 1.2 to 1.6 of 1.965
+// GHz, so their time is their energy.  131,072 x 768 x 1,152 bf16 with bias and residual takes 235 us (990
+// TFLOP/s), 178 us of it with the drain left out; 16,384 x 4,096 x 4,096 e4m3 with erf-GELU, bias and
+// residual 265 us (2.07 PFLOP/s; plain 229 us); gated int8 131,072 x 1,152 x 768 240 us (1.93 POP/s), 163 us
+// without the drain.  The operands' way into shared memory comes next: 32 KB per CTA and K step of 512 MMA
+// cycles.  Below one wave of tiles the time is latency: launch, one load, the K steps, the drain.
+//
+// The drain's shape was measured: its warps must not wait for one another (a barrier per tile among 16 warps
+// with common column values: 1.18 times the time on plain bf16 131,072 x 768 x 1,152; 8 warps with values of
+// their own: 1.03 times glp_bf16_gemm's, which has no epilogue), must release the accumulator as soon as it
+// is read (gated int8: 236 us, 252 us after the stores), and needs few instructions rather than few special
+// functions (one reciprocal for two outputs: 265 us instead of 236).
 #pragma once
 #include "common.cuh"
 #include "linear.cuh"
@@ -39,7 +53,7 @@ struct LinearTcCfg {
   static constexpr int OUT_N = GATED ? BN / 2 : BN;  // output columns per tile
   static constexpr int EPI_WARPS = EPI;
   static constexpr int W = 4 * OUT_N / EPI;          // output columns per epilogue warp
-  static constexpr int CH = GATED && EPI == 16 ? 16 : 32;   // ... drained at a time
+  static constexpr int CH = GATED && EPI == 16 ? 16 : 32;  // ... drained at a time (96 registers with 16 warps)
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int STAGES = BN == 64 ? 6 : (EPI == 16 ? 4 : 5);
   static constexpr uint32_t A_BYTES = 128 * 128;
@@ -74,8 +88,8 @@ __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint
 #undef GLP_UMMA
 }
 
-// 16 / 32 consecutive accumulator columns, and the wait for one or two such loads that also names their
-// registers, so that no use of them is scheduled before it
+// 16 / 32 consecutive accumulator columns, and the wait for such loads that also names their registers, so
+// that no use of them is scheduled before it
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(

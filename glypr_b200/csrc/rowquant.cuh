@@ -4,7 +4,11 @@
 //   x~ = x * rms(x) * post_gain   (or x),   h = (residual + x~) * layer_scalar,
 //   n  = h * rms(h) * gain,   scale = max(max|n| / top, 2^-100),   code = rn(n / scale)
 //
-// Everything between the loads and the two roundings (h to its type, n to its code) is f32.
+// Everything between the loads and the two roundings (h to its type, n to its code) is f32, and a row stays
+// in registers from its one read to its one write.  Whole chunks of 8 elements are bound by memory: 262,144 x
+// 768 (f16 + bf16 residual, both norms) 241 to 251 us = 5.6 to 5.9 TB/s, 131,072 x 1,152 f16 quantised 75 us =
+// 6.0 TB/s, 32,768 x 4,096 norm 141 us = 6.6 TB/s (a copy: 6.5).  Rows that start anywhere are bound by
+// instructions (the gains' shift, the rows' ends): 10,007 x 1,543 norm 34 us = 3.2 TB/s.
 #pragma once
 #include "common.cuh"
 

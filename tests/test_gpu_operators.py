@@ -512,6 +512,27 @@ def test_linear_output_past_32_bit_offsets():
     c.check(slice(0, 70))
 
 
+@pytest.mark.parametrize("m,n", [(540_000, 24), (3, 540_000), (300, 540_000)])
+def test_linear_operands_past_32_bit_offsets(m, n):
+    """x or w of more than 2^31 elements: each kernel's last rows and columns."""
+    k = 4000
+    c = Case.__new__(Case)
+    c.m, c.n, c.k, c.dtype, c.out, c.act = m, n, k, "i8", "f32", "none"
+    c.x = torch.zeros((m, k), dtype=torch.int8, device="cuda")
+    c.w = torch.zeros((n, k), dtype=torch.int8, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m + n)
+    for t in (c.x, c.w):
+        tail = t[-2000:]
+        tail.copy_(torch.randint(-127, 128, tail.shape, generator=g, device="cuda", dtype=torch.int8))
+    c.xs = c.ws = c.wus = c.wu = c.b = c.bu = c.res = None
+    c.y = torch.full((m, n), float("nan"), device="cuda")
+    c.run()
+    want = (c.x[-2000:].double() @ c.w[-2000:].double().T).float()
+    assert torch.equal(c.y[-2000:, -2000:], want)
+    assert not c.y.isnan().any()
+
+
 def test_zero_rows_are_a_no_op():
     api.linear(0, 8, 8, DT["f16"], 0, 0, 0, DT["f16"])
     api.quantize_rows(0, 8, 0, DT["f16"], 0, DT["i8"], 0)
