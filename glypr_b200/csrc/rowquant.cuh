@@ -98,6 +98,17 @@ __device__ __forceinline__ float scale_of(float amax, int q_dtype) {
   return s < kQuantFloor ? kQuantFloor : s;
 }
 
+// rms(v) from the sum of squares
+__device__ __forceinline__ float inv_rms(float ss, const RowQuantParams& p) { return rsqrtf(fmaf(ss, p.inv_H, p.eps)); }
+
+// The factor from values to codes: top / amax by one rounded quotient (the rms and the scale's own rounding
+// cancel in it), and 1 / scale where the scale is the floor.  With the quotient of the rounded rms and scale
+// in its place three times as many codes fell on the other side of a rounding boundary.
+__device__ __forceinline__ float code_factor(float amax, float inv, float s, int q_dtype) {
+  const bool above = s > kQuantFloor;  // (a scale of NaN: whatever the code)
+  return (above ? quant_top(q_dtype) : inv) / (above ? amax : s);
+}
+
 // One element at a time, any alignment: G threads per row, NC elements per thread, H <= G * NC.
 // NORM false: plain row quantisation.
 template <int G, int NC, bool NORM>
@@ -122,7 +133,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
 #pragma unroll
       for (int c = 0; c < NC; ++c) ss = fmaf(v[c], v[c], ss);
       row_reduce<G>(ss, none);
-      inv = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+      inv = inv_rms(ss, p);
     }
     float ss = 0.0f, amax = 0.0f;
 #pragma unroll
@@ -140,9 +151,9 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
       }
     }
     row_reduce<G>(ss, amax);
-    const float inv_h = 1.0f / sqrtf(ss / static_cast<float>(p.H) + p.eps);
+    const float inv_h = inv_rms(ss, p);
     const float s = scale_of(amax * inv_h, p.q_dtype);
-    const float k = inv_h / s;
+    const float k = code_factor(amax, inv_h, s, p.q_dtype);
     if (t == 0) p.scale[row] = s;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -354,9 +365,6 @@ __device__ __forceinline__ float f2_hsum(uint64_t v) {
   return lo + hi;
 }
 
-// rms(v) from the sum of squares
-__device__ __forceinline__ float inv_rms(float ss, const RowQuantParams& p) { return rsqrtf(fmaf(ss, p.inv_H, p.eps)); }
-
 // G threads per row, NC chunks per thread: the row touches at most G NC chunks.  XT, HT: types of x and
 // of residual / h.  gains16: both gains start on 16-byte boundaries.  PLACE
 // kFlush and kFull also promise gains16.
@@ -432,7 +440,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQ
     row_reduce<G, true, true>(ss, amax);
     const float inv_h = inv_rms(ss, p);
     const float s = scale_of(amax * inv_h, p.q_dtype);
-    const float k = __fdividef(inv_h, s);
+    const float k = code_factor(amax, inv_h, s, p.q_dtype);
     if (t == 0) p.scale[row] = s;
 #pragma unroll
     for (int c = 0; c < NC; ++c) store_codes<PLACE>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
