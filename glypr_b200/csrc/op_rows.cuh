@@ -15,9 +15,9 @@ int launch_quant_chunks(const RowQuantParams& p, cudaStream_t st);
 
 template <int G, int NC, int XT, int HT, bool NORM, int PLACE>
 int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
-  constexpr int ROWS = G == 32 ? 8 : 1;
+  constexpr int ROWS = G <= 32 ? 256 / G : 1;
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.M) + ROWS - 1) / ROWS);
-  return launch(row_quant_kernel<G, NC, XT, HT, NORM, PLACE>, grid, G == 32 ? 256 : G, 0, 1, st, p, gains16);
+  return launch(row_quant_kernel<G, NC, XT, HT, NORM, PLACE>, grid, G <= 32 ? 256 : G, 0, 1, st, p, gains16);
 }
 
 // How many chunks of 8 the row touches, from a chunk's start or not.
@@ -34,6 +34,7 @@ inline int chunks_of(const RowQuantParams& p, bool* flush) {
 // they fill: 32,768 x 5,000 quantisation 80 us, 170 us with 512 threads of 2 chunks.
 template <int XT, int HT, bool NORM, int PLACE>
 int launch_width(const RowQuantParams& p, int chunks, bool gains16, cudaStream_t st) {
+  if (chunks <= 16) return launch_chunks<16, 1, XT, HT, NORM, PLACE>(p, gains16, st);
   if (chunks <= 32) return launch_chunks<32, 1, XT, HT, NORM, PLACE>(p, gains16, st);
   if (chunks <= 64) return launch_chunks<32, 2, XT, HT, NORM, PLACE>(p, gains16, st);
   if (chunks <= 96) return launch_chunks<32, 3, XT, HT, NORM, PLACE>(p, gains16, st);

@@ -67,13 +67,15 @@ __device__ __forceinline__ uint8_t code_of(float v, int q_dtype) {
   return q_dtype == kI8 ? code_i8(v) : static_cast<uint8_t>(code_e4m3x2(v, 0.0f));
 }
 
-// sum of a (SUM) and NaN-keeping maximum of b (MAX) over the G threads that share a row (a warp or the block)
+// sum of a (SUM) and NaN-keeping maximum of b (MAX) over the G threads that share a row (16 lanes, a warp or
+// the block)
 template <int G, bool SUM = true, bool MAX = true>
 __device__ __forceinline__ void row_reduce(float& a, float& b) {
+  const uint32_t lanes = G >= 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    if constexpr (SUM) a += __shfl_xor_sync(0xffffffffu, a, o);
-    if constexpr (MAX) b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+  for (int o = G >= 32 ? 16 : G / 2; o > 0; o >>= 1) {
+    if constexpr (SUM) a += __shfl_xor_sync(lanes, a, o);
+    if constexpr (MAX) b = max_nan(b, __shfl_xor_sync(lanes, b, o));
   }
   if constexpr (G > 32) {
     __shared__ float2 part[G / 32];
@@ -369,13 +371,13 @@ __device__ __forceinline__ float f2_hsum(uint64_t v) {
 // of residual / h.  gains16: both gains start on 16-byte boundaries.  PLACE
 // kFlush and kFull also promise gains16.
 template <int G, int NC, int XT, int HT, bool NORM, int PLACE>
-__global__ void __launch_bounds__(G == 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
-  constexpr int ROWS = G == 32 ? 8 : 1;
+__global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
+  constexpr int ROWS = G <= 32 ? 256 / G : 1;
   const int t = threadIdx.x % G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G;
   griddep_launch();
   griddep_wait();
-  if (row >= p.M) return;  // whole warps or the whole block
+  if (row >= p.M) return;  // the row's threads together
   const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * kBytes<XT>;
   const int off = PLACE != kShifted ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
   Chunk<XT> xc[NC];

@@ -162,7 +162,7 @@ def norm_want(x, res, post, gain, scalar):
                              .clamp_min(1e-300)) * (1 if gain is None else gain.abs())
 
 
-@pytest.mark.parametrize("h", [1, 5, 64, 256, 512, 768, 1024, 1152, 1543, 2048, 2568, 4096, 5000, 6000, 8000, 9001,
+@pytest.mark.parametrize("h", [1, 5, 64, 117, 256, 512, 768, 1024, 1152, 1543, 2048, 2568, 4096, 5000, 6000, 8000, 9001,
                                12000, 16384, 20004, 32761, 32768])
 @pytest.mark.parametrize("xd,hd,qd", [("f16", "bf16", "i8"), ("bf16", "bf16", "e4m3"), ("f32", "f32", "i8"),
                                       ("f16", "f32", "e4m3"), ("f32", "f16", "e4m3")])
