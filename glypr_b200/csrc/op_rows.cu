@@ -22,8 +22,7 @@ bool same_chunks(const RowQuantParams& p) {
 
 template <bool NORM>
 int launch_row_quant(const RowQuantParams& p, cudaStream_t st) {
-  const bool at_chunk = reinterpret_cast<uintptr_t>(p.x) / dtype_size(p.x_dtype) % 8 == 0 && p.ld_x % 8 == 0;
-  if (same_chunks(p) && (at_chunk || (p.H + 14) / 8 <= GLP_QUANT_MAX_H / 8)) {  // (else one chunk too many)
+  if (same_chunks(p)) {
     if constexpr (NORM) {
       const bool gains16 = aligned(p.gain, 16) && aligned(p.post_gain, 16);
       if (p.x_dtype == GLP_DTYPE_F32) return launch_norm_chunks<glp::kF32>(p, gains16, st);

@@ -20,23 +20,17 @@ int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
   return launch(row_quant_kernel<G, NC, XT, HT, NORM, PLACE>, grid, G <= 32 ? 256 : G, 0, 1, st, p, gains16);
 }
 
-// How many chunks of 8 the row touches, from a chunk's start or not.
-inline int chunks_of(const RowQuantParams& p, bool* flush) {
-  *flush = reinterpret_cast<uintptr_t>(p.x) / dtype_size(p.x_dtype) % 8 == 0 && p.ld_x % 8 == 0;
-  const int chunks = (p.H + (*flush ? 7 : 14)) / 8;
-  *flush = *flush && p.H % 8 == 0;
-  return chunks;
-}
-
-// A warp per row while a lane's chunks stay few (no block-wide reductions); past that 128 threads: 32,768 x
+// The fewest lanes whose chunks stay few: 8 up to 256 elements (262,144 x 64 norm 25 us, 41 us with 16 lanes,
+// 262,144 x 160 65 us, 81 us with a warp), a warp up to 1,280; past that 128 threads: 32,768 x
 // 2,008 bf16 with both norms 99 us, 122 us with a warp per row; row quantisation, which holds half as much,
 // 32,768 x 1,537 38 us with a warp, 45 us with 128 threads.  Wider rows take the smallest block whose chunks
 // they fill: 32,768 x 5,000 quantisation 80 us, 170 us with 512 threads of 2 chunks.
 template <int XT, int HT, bool NORM, int PLACE>
 int launch_width(const RowQuantParams& p, int chunks, bool gains16, cudaStream_t st) {
-  if (chunks <= 16) return launch_chunks<16, 1, XT, HT, NORM, PLACE>(p, gains16, st);
-  if (chunks <= 32) return launch_chunks<32, 1, XT, HT, NORM, PLACE>(p, gains16, st);
-  if (chunks <= 64) return launch_chunks<32, 2, XT, HT, NORM, PLACE>(p, gains16, st);
+  if (chunks <= 8) return launch_chunks<8, 1, XT, HT, NORM, PLACE>(p, gains16, st);
+  if (chunks <= 16) return launch_chunks<8, 2, XT, HT, NORM, PLACE>(p, gains16, st);
+  if (chunks <= 32) return launch_chunks<8, 4, XT, HT, NORM, PLACE>(p, gains16, st);
+  if (chunks <= 64) return launch_chunks<16, 4, XT, HT, NORM, PLACE>(p, gains16, st);
   if (chunks <= 96) return launch_chunks<32, 3, XT, HT, NORM, PLACE>(p, gains16, st);
   if (chunks <= 128) return launch_chunks<32, 4, XT, HT, NORM, PLACE>(p, gains16, st);
   if (chunks <= 160) return launch_chunks<32, 5, XT, HT, NORM, PLACE>(p, gains16, st);
@@ -57,8 +51,8 @@ int launch_width(const RowQuantParams& p, int chunks, bool gains16, cudaStream_t
 
 template <int XT, int HT, bool NORM>
 int launch_place(const RowQuantParams& p, bool gains16, cudaStream_t st) {
-  bool flush;
-  const int chunks = chunks_of(p, &flush);
+  const int chunks = p.H / 8;
+  const bool flush = reinterpret_cast<uintptr_t>(p.x) / dtype_size(p.x_dtype) % 8 == 0 && p.ld_x % 8 == 0 && p.H % 8 == 0;
   if (!flush || !gains16) return launch_width<XT, HT, NORM, kShifted>(p, chunks, gains16, st);
   if (chunks == 64) return launch_chunks<32, 2, XT, HT, NORM, kFull>(p, gains16, st);
   if (chunks == 96) return launch_chunks<32, 3, XT, HT, NORM, kFull>(p, gains16, st);

@@ -67,11 +67,11 @@ __device__ __forceinline__ uint8_t code_of(float v, int q_dtype) {
   return q_dtype == kI8 ? code_i8(v) : static_cast<uint8_t>(code_e4m3x2(v, 0.0f));
 }
 
-// sum of a (SUM) and NaN-keeping maximum of b (MAX) over the G threads that share a row (16 lanes, a warp or
-// the block)
+// sum of a (SUM) and NaN-keeping maximum of b (MAX) over the G threads that share a row (8 or 16 lanes, a
+// warp or the block)
 template <int G, bool SUM = true, bool MAX = true>
 __device__ __forceinline__ void row_reduce(float& a, float& b) {
-  const uint32_t lanes = G >= 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+  const uint32_t lanes = G >= 32 ? 0xffffffffu : ((1u << (G & 31)) - 1) << (threadIdx.x & 31 & ~(G - 1));
 #pragma unroll
   for (int o = G >= 32 ? 16 : G / 2; o > 0; o >>= 1) {
     if constexpr (SUM) a += __shfl_xor_sync(lanes, a, o);
@@ -181,16 +181,10 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
 // ---------------------------------------------------------------------------- 8 elements at a time
 // The same rows in aligned chunks of 8 elements (one 16-byte load of a 16-bit row, two of an f32 row,
 // one 8-byte store of codes).  Rows need not start on a chunk boundary -- a packed odd width has no two
-// rows alike -- as long as x, residual, h and q all stand at the same place in their chunks: chunk i of
-// a row is elements [8 i - off, 8 i - off + 8), and only the two at the row's ends go by element.
-// how a row lies in its chunks: anywhere; from a chunk's start, in whole chunks; and exactly as many as
-// its threads hold
-constexpr int kShifted = 0, kFlush = 1, kFull = 2;
-template <int PLACE>
-__device__ __forceinline__ bool whole_chunk(int e, int H) {
-  return PLACE == kFull || (PLACE == kFlush ? e < H : e >= 0 && e + 8 <= H);
-}
-
+// rows alike -- as long as x, residual, h and q all stand at the same place in their chunks: the row is
+// then `head` elements up to its first boundary, whole chunks, and a tail, and the at most 14 elements of
+// head and tail go one per lane beside the chunks (by element in the lane that holds the chunk they cost
+// more than all the chunks: 131,072 x 250 norm 154 us).
 template <int DT>
 constexpr int kBytes = DT == kF32 ? 4 : 2;
 
@@ -205,31 +199,13 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no li
   return v;
 }
 
-// elements [e, e + 8) of the row at `row`, zeros outside [0, H)
-template <int DT, int PLACE>
-__device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, int H) {
+// elements [e, e + 8) of the row at `row`, zeros for no chunk
+template <int DT>
+__device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, bool on) {
   constexpr int B = kBytes<DT>;
   Chunk<DT> c;
-  if (whole_chunk<PLACE>(e, H)) {
 #pragma unroll
-    for (int i = 0; i < B / 2; ++i) c.v[i] = ld_stream(row + static_cast<int64_t>(e) * B + 16 * i);
-  } else {
-    uint32_t w[2 * B];
-#pragma unroll
-    for (int i = 0; i < 2 * B; ++i) w[i] = 0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int n = e + j;
-      if (PLACE == kShifted && n >= 0 && n < H) {
-        if constexpr (B == 4)
-          w[j] = *reinterpret_cast<const uint32_t*>(row + static_cast<int64_t>(n) * 4);
-        else
-          w[j / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + static_cast<int64_t>(n) * 2)) << (16 * (j & 1));
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < B / 2; ++i) c.v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-  }
+  for (int i = 0; i < B / 2; ++i) c.v[i] = on ? ld_stream(row + static_cast<int64_t>(e) * B + 16 * i) : make_uint4(0u, 0u, 0u, 0u);
   return c;
 }
 
@@ -250,39 +226,33 @@ __device__ __forceinline__ void chunk_f32(const Chunk<DT>& c, uint64_t (&v)[4]) 
   }
 }
 
-template <int DT, int PLACE>
-__device__ __forceinline__ void store_chunk(uint8_t* row, int e, int H, const uint64_t (&p)[4]) {
+template <int DT>
+__device__ __forceinline__ void store_chunk(uint8_t* row, int e, bool on, const uint64_t (&p)[4]) {
   constexpr int B = kBytes<DT>;
+  if (!on) return;
   float v[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) f2_split(p[j], v[2 * j], v[2 * j + 1]);
-  if (whole_chunk<PLACE>(e, H)) {
-    uint8_t* at = row + static_cast<int64_t>(e) * B;
-    if constexpr (B == 4) {
-      *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(at + 16) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
+  uint8_t* at = row + static_cast<int64_t>(e) * B;
+  if constexpr (B == 4) {
+    *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(at + 16) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (DT == kBF16) {
-          w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-        } else {
-          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == kBF16) {
+        w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+      } else {
+        const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-  } else if (PLACE == kShifted) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (e + j >= 0 && e + j < H) store_from_f32(row, e + j, DT, v[j]);
+    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-template <int PLACE>
-__device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dtype, const uint64_t (&p)[4], uint64_t k) {
+__device__ __forceinline__ void store_codes(uint8_t* row, int e, bool on, int q_dtype, const uint64_t (&p)[4], uint64_t k) {
   uint32_t w[2];
   if (q_dtype == kI8) {
     // v * k + 1.5 * 2^23 rounds once to the nearest integer, ties to even, and leaves it in the low byte
@@ -305,13 +275,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int e, int H, int q_dt
     w[0] = __byte_perm(h[0], h[1], 0x5410);
     w[1] = __byte_perm(h[2], h[3], 0x5410);
   }
-  if (whole_chunk<PLACE>(e, H)) {
-    *reinterpret_cast<uint2*>(row + e) = make_uint2(w[0], w[1]);
-  } else if (PLACE == kShifted) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (e + j >= 0 && e + j < H) row[e + j] = static_cast<uint8_t>(w[j / 4] >> (8 * (j & 3)));
-  }
+  if (on) *reinterpret_cast<uint2*>(row + e) = make_uint2(w[0], w[1]);
 }
 
 // largest magnitude of m and 8 values, keeping a NaN
@@ -325,29 +289,34 @@ __device__ __forceinline__ float max8(float m, const uint64_t (&p)[4]) {
   return m;
 }
 
-// gain[e .. e + 8) (outside [0, H) any finite value).  e is a multiple of 8 less the row's off: for an
-// unaligned row the aligned words around it are loaded and shifted by off & 3, the same for the whole row.
-template <int PLACE>
-__device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, int H, uint64_t (&p)[4]) {
-  if (PLACE != kShifted && e >= H) {  // (only where the chunk is empty: its values are zeros)
+// gain[e .. e + 8), zeros for no chunk.  From an unaligned e the aligned words around it are loaded and
+// shifted by e & 3, which is the same for the whole row.
+template <bool SHIFTED>
+__device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int e, bool on, uint64_t (&p)[4]) {
+  if (!on) {
     p[0] = p[1] = p[2] = p[3] = f2(0.0f, 0.0f);
     return;
   }
-  const int s = e & 3;
-  if (PLACE != kShifted || (aligned16 && s == 0 && e >= 0 && e + 8 <= H)) {
+  const int s = SHIFTED ? e & 3 : 0;
+  if (!SHIFTED || (aligned16 && s == 0)) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(gain + e)), b = __ldg(reinterpret_cast<const float4*>(gain + e) + 1);
     p[0] = f2(a.x, a.y), p[1] = f2(a.z, a.w), p[2] = f2(b.x, b.y), p[3] = f2(b.z, b.w);
     return;
   }
   float v[8];
-  if (aligned16 && e - s >= 0 && e - s + 12 <= H) {
+  if (aligned16) {
     float w[12];
     const float4* at = reinterpret_cast<const float4*>(gain + (e - s));
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const float4 f = __ldg(at + i);
       w[4 * i] = f.x, w[4 * i + 1] = f.y, w[4 * i + 2] = f.z, w[4 * i + 3] = f.w;
     }
+    // (the s values that the third word is needed for; the row may end with them)
+    w[8] = __ldg(gain + (e - s + 8));
+    w[9] = s > 1 ? __ldg(gain + (e - s + 9)) : 0.0f;
+    w[10] = s > 2 ? __ldg(gain + (e - s + 10)) : 0.0f;
+    w[11] = 0.0f;
     // a shift by s in two steps, so that every index is known at compile time
 #pragma unroll
     for (int j = 0; j < 10; ++j) w[j] = s & 2 ? w[j + 2] : w[j];
@@ -355,7 +324,7 @@ __device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int
     for (int j = 0; j < 8; ++j) v[j] = s & 1 ? w[j + 1] : w[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = e + j >= 0 && e + j < H ? __ldg(gain + e + j) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = __ldg(gain + e + j);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) p[j] = f2(v[2 * j], v[2 * j + 1]);
@@ -367,32 +336,70 @@ __device__ __forceinline__ float f2_hsum(uint64_t v) {
   return lo + hi;
 }
 
-// G threads per row, NC chunks per thread: the row touches at most G NC chunks.  XT, HT: types of x and
-// of residual / h.  gains16: both gains start on 16-byte boundaries.  PLACE
-// kFlush and kFull also promise gains16.
+// how a row lies in its chunks: anywhere; from a chunk's start, in whole chunks; and exactly as many as
+// its threads hold
+constexpr int kShifted = 0, kFlush = 1, kFull = 2;
+
+// G threads per row, NC chunks per thread: a row has at most G NC whole chunks.  XT, HT: types of x and of
+// residual / h.  gains16: both gains start on 16-byte boundaries (kFlush and kFull promise it).
 template <int G, int NC, int XT, int HT, bool NORM, int PLACE>
 __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
   constexpr int ROWS = G <= 32 ? 256 / G : 1;
+  constexpr bool SHIFTED = PLACE == kShifted;
+  constexpr int ED = !SHIFTED ? 0 : (G >= 16 ? 1 : 2);  // head and tail elements per lane
   const int t = threadIdx.x % G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / G;
   griddep_launch();
   griddep_wait();
   if (row >= p.M) return;  // the row's threads together
   const uint8_t* xr = static_cast<const uint8_t*>(p.x) + row * p.ld_x * kBytes<XT>;
-  const int off = PLACE != kShifted ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7);
-  Chunk<XT> xc[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT, PLACE>(xr, (c * G + t) * 8 - off, p.H);
   uint8_t* qr = static_cast<uint8_t*>(p.q) + row * p.ld_q;
+  const int off = SHIFTED ? static_cast<int>(reinterpret_cast<uintptr_t>(xr) / kBytes<XT> & 7) : 0;
+  const int head = SHIFTED && off ? min(8 - off, p.H) : 0;
+  const int chunks = (p.H - head) / 8;
+  const auto e_of = [&](int c) { return head + (c * G + t) * 8; };
+  const auto on = [&](int c) { return PLACE == kFull || c * G + t < chunks; };
+  // this lane's elements of head and tail
+  int ne[ED ? ED : 1];
+  bool oe[ED ? ED : 1];
+#pragma unroll
+  for (int d = 0; d < ED; ++d) {
+    const bool last = G >= 16 ? t >= 8 : d == 1;
+    const int j = t & 7, from = head + chunks * 8;
+    ne[d] = last ? from + j : j;
+    oe[d] = t < 16 && (last ? from + j < p.H : j < head);
+  }
+  Chunk<XT> xc[NC];
+  float ve[ED ? ED : 1];
+#pragma unroll
+  for (int d = 0; d < ED; ++d) ve[d] = oe[d] ? load_as_f32(xr, ne[d], XT) : 0.0f;
   uint64_t v[NC][4];
   float none = 0.0f, amax = 0.0f;
   if constexpr (NORM) {
     const uint8_t* rr = static_cast<const uint8_t*>(p.residual) + row * p.ld_residual * kBytes<HT>;
     uint8_t* hr = static_cast<uint8_t*>(p.h) + row * p.ld_h * kBytes<HT>;
     Chunk<HT> rc[NC];
+    float re[ED ? ED : 1];
+    // Full rows: x and residual side by side, for which the compiler takes more registers and keeps more in
+    // flight (131,072 x 512: 86 us, 95 us with x first); the other kinds are slower with it (65,536 x 1,152:
+    // 115 us, 101 us).
+    if constexpr (PLACE == kFull) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        xc[c] = load_chunk<XT>(xr, e_of(c), true);
+        if (p.residual) rc[c] = load_chunk<HT>(rr, e_of(c), true);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, e_of(c), on(c));
+      if (p.residual) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT>(rr, e_of(c), on(c));
+      }
+    }
     if (p.residual) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT, PLACE>(rr, (c * G + t) * 8 - off, p.H);
+      for (int d = 0; d < ED; ++d) re[d] = oe[d] ? load_as_f32(rr, ne[d], HT) : 0.0f;
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) chunk_f32<XT>(xc[c], v[c]);
@@ -404,18 +411,22 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss2 = f2_fma(v[c][j], v[c][j], ss2);
       float ss = f2_hsum(ss2);
+#pragma unroll
+      for (int d = 0; d < ED; ++d) ss = fmaf(ve[d], ve[d], ss);
       row_reduce<G, true, false>(ss, none);
       const float inv = inv_rms(ss, p);
       inv2 = f2(inv, inv);
+#pragma unroll
+      for (int d = 0; d < ED; ++d) ve[d] = ve[d] * inv * (oe[d] ? __ldg(p.post_gain + ne[d]) : 0.0f);
     }
     const uint64_t scalar2 = f2(p.layer_scalar, p.layer_scalar);
     uint64_t ss2 = f2(0.0f, 0.0f);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int e = (c * G + t) * 8 - off;
+      const int e = e_of(c);
       uint64_t g[4];
       if (p.post_gain) {
-        load_gain<PLACE>(p.post_gain, gains16, e, p.H, g);
+        load_gain<SHIFTED>(p.post_gain, gains16, e, on(c), g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(f2_mul(v[c][j], inv2), g[j]);
       }
@@ -430,34 +441,53 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
         v[c][j] = f2_mul(v[c][j], scalar2);
         ss2 = f2_fma(v[c][j], v[c][j], ss2);
       }
-      if (p.h) store_chunk<HT, PLACE>(hr, e, p.H, v[c]);
+      if (p.h) store_chunk<HT>(hr, e, on(c), v[c]);
       if (p.gain) {
-        load_gain<PLACE>(p.gain, gains16, e, p.H, g);
+        load_gain<SHIFTED>(p.gain, gains16, e, on(c), g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(v[c][j], g[j]);
       }
       amax = max8(amax, v[c]);
     }
     float ss = f2_hsum(ss2);
+#pragma unroll
+    for (int d = 0; d < ED; ++d) {
+      if (p.residual) ve[d] += re[d];
+      ve[d] *= p.layer_scalar;
+      ss = fmaf(ve[d], ve[d], ss);
+      if (p.h && oe[d]) store_from_f32(hr, ne[d], HT, ve[d]);
+      if (p.gain) ve[d] *= oe[d] ? __ldg(p.gain + ne[d]) : 0.0f;
+      amax = max_nan(amax, fabsf(ve[d]));
+    }
     row_reduce<G, true, true>(ss, amax);
     const float inv_h = inv_rms(ss, p);
     const float s = scale_of(amax * inv_h, p.q_dtype);
     const float k = code_factor(amax, inv_h, s, p.q_dtype);
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes<PLACE>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
+    for (int c = 0; c < NC; ++c) store_codes(qr, e_of(c), on(c), p.q_dtype, v[c], f2(k, k));
+#pragma unroll
+    for (int d = 0; d < ED; ++d)
+      if (oe[d]) qr[ne[d]] = code_of(ve[d] * k, p.q_dtype);
   } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, e_of(c), on(c));
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       chunk_f32<XT>(xc[c], v[c]);
       amax = max8(amax, v[c]);
     }
+#pragma unroll
+    for (int d = 0; d < ED; ++d) amax = max_nan(amax, fabsf(ve[d]));
     row_reduce<G, false, true>(none, amax);
     const float s = scale_of(amax, p.q_dtype);
     const float k = 1.0f / s;
     if (t == 0) p.scale[row] = s;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) store_codes<PLACE>(qr, (c * G + t) * 8 - off, p.H, p.q_dtype, v[c], f2(k, k));
+    for (int c = 0; c < NC; ++c) store_codes(qr, e_of(c), on(c), p.q_dtype, v[c], f2(k, k));
+#pragma unroll
+    for (int d = 0; d < ED; ++d)
+      if (oe[d]) qr[ne[d]] = code_of(ve[d] * k, p.q_dtype);
   }
 }
 
