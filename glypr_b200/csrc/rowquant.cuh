@@ -370,6 +370,10 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
     oe[d] = t < 16 && (last ? from + j < p.H : j < head);
   }
   Chunk<XT> xc[NC];
+  if constexpr (!NORM || PLACE != kFull) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, e_of(c), on(c));
+  }
   float ve[ED ? ED : 1];
 #pragma unroll
   for (int d = 0; d < ED; ++d) ve[d] = oe[d] ? load_as_f32(xr, ne[d], XT) : 0.0f;
@@ -381,21 +385,17 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
     Chunk<HT> rc[NC];
     float re[ED ? ED : 1];
     // Full rows: x and residual side by side, for which the compiler takes more registers and keeps more in
-    // flight (131,072 x 512: 86 us, 95 us with x first); the other kinds are slower with it (65,536 x 1,152:
-    // 115 us, 101 us).
+    // flight (131,072 x 512: 86 us, 95 us with x first); the other kinds, whose x is on its way by now, are
+    // slower with it (65,536 x 1,152: 115 us, 101 us).
     if constexpr (PLACE == kFull) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         xc[c] = load_chunk<XT>(xr, e_of(c), true);
         if (p.residual) rc[c] = load_chunk<HT>(rr, e_of(c), true);
       }
-    } else {
+    } else if (p.residual) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, e_of(c), on(c));
-      if (p.residual) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT>(rr, e_of(c), on(c));
-      }
+      for (int c = 0; c < NC; ++c) rc[c] = load_chunk<HT>(rr, e_of(c), on(c));
     }
     if (p.residual) {
 #pragma unroll
@@ -470,8 +470,6 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
     for (int d = 0; d < ED; ++d)
       if (oe[d]) qr[ne[d]] = code_of(ve[d] * k, p.q_dtype);
   } else {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) xc[c] = load_chunk<XT>(xr, e_of(c), on(c));
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       chunk_f32<XT>(xc[c], v[c]);
