@@ -22,9 +22,9 @@ int launch_chunks(const RowQuantParams& p, bool gains16, cudaStream_t st) {
 
 // The fewest lanes whose chunks stay few: 8 up to 256 elements (262,144 x 64 norm 25 us, 41 us with 16 lanes,
 // 262,144 x 160 65 us, 81 us with a warp), a warp up to 1,280; past that 128 threads: 32,768 x
-// 2,008 bf16 with both norms 99 us, 122 us with a warp per row; row quantisation, which holds half as much,
-// 32,768 x 1,537 38 us with a warp, 45 us with 128 threads.  Wider rows take the smallest block whose chunks
-// they fill: 32,768 x 5,000 quantisation 80 us, 170 us with 512 threads of 2 chunks.
+// 2,008 bf16 with both norms 93 us, 122 us with a warp per row; row quantisation, which holds half as much,
+// 32,768 x 1,537 27 us with a warp (128 threads took a fifth more).  Wider rows take the smallest block whose chunks
+// they fill: 32,768 x 5,000 quantisation 76 us, 170 us with 512 threads of 2 chunks.
 template <int XT, int HT, bool NORM, int PLACE>
 int launch_width(const RowQuantParams& p, int chunks, bool gains16, cudaStream_t st) {
   if (chunks <= 8) return launch_chunks<8, 1, XT, HT, NORM, PLACE>(p, gains16, st);

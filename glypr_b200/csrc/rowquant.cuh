@@ -6,9 +6,11 @@
 //
 // Everything between the loads and the two roundings (h to its type, n to its code) is f32, and a row stays
 // in registers from its one read to its one write.  Whole chunks of 8 elements are bound by memory: 262,144 x
-// 768 (f16 + bf16 residual, both norms) 241 to 251 us = 5.6 to 5.9 TB/s, 131,072 x 1,152 f16 quantised 75 us =
-// 6.0 TB/s, 32,768 x 4,096 norm 141 us = 6.6 TB/s (a copy: 6.5).  Rows that start anywhere are bound by
-// instructions (the gains' shift, the rows' ends): 10,007 x 1,543 norm 34 us = 3.2 TB/s.
+// 768 (f16 + bf16 residual, both norms) 250 us = 5.6 TB/s, 131,072 x 1,152 f16 quantised 75 us = 6.0 TB/s,
+// 32,768 x 4,096 norm 149 us = 6.3 TB/s (a copy: 6.5).  Rows that start anywhere take a third more
+// instructions (the gains' shift, head and tail): 10,007 x 1,543 norm 28.4 us = 3.8 TB/s, 65,536 x 771 118 us =
+// 4.7 TB/s.  Tried and slower: gains kept in registers over a block's rows (10,007 x 1,543 56 us: fewer warps),
+// edge chunks read whole and masked (34 us), a shared-memory pass is not shorter in instructions.
 #pragma once
 #include "common.cuh"
 
@@ -108,7 +110,8 @@ __device__ __forceinline__ float inv_rms(float ss, const RowQuantParams& p) { re
 // in its place three times as many codes fell on the other side of a rounding boundary.
 __device__ __forceinline__ float code_factor(float amax, float inv, float s, int q_dtype) {
   const bool above = s > kQuantFloor;  // (a scale of NaN: whatever the code)
-  return (above ? quant_top(q_dtype) : inv) / (above ? amax : s);
+  // finite, so that zeros keep code 0 also where eps is so small that 1 / (rms scale) overflows
+  return fminf((above ? quant_top(q_dtype) : inv) / (above ? amax : s), 3.4028235e38f);
 }
 
 // One element at a time, any alignment: G threads per row, NC elements per thread, H <= G * NC.
@@ -479,6 +482,8 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
     for (int d = 0; d < ED; ++d) amax = max_nan(amax, fabsf(ve[d]));
     row_reduce<G, false, true>(none, amax);
     const float s = scale_of(amax, p.q_dtype);
+    // (v * k is within an ulp of v / s; the rounded quotient, a correction more, gave no fewer codes beyond a
+    // rounding boundary -- the scale itself is rounded -- and took 80 us instead of 74 for 131,072 x 1,152)
     const float k = 1.0f / s;
     if (t == 0) p.scale[row] = s;
 #pragma unroll

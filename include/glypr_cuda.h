@@ -359,8 +359,8 @@ int glp_flash_attention(const void* d_qkv, const int32_t* d_cu_seqlens, int n_se
 
 #define GLP_QUANT_MAX_H 32768 /* longest row of the two quantising entry points */
 
-/* A row's 8-bit form: scale = max(max|v| / top, 2^-100), code = v / scale rounded to the nearest
- * code (ties to even); top = 127 (GLP_DTYPE_I8) or 448 (GLP_DTYPE_E4M3), so code * scale is the
+/* A row's 8-bit form: scale = max(max|v| / top, 2^-100), code = v / scale (in f32, to an ulp)
+ * rounded to the nearest code, ties to even; top = 127 (GLP_DTYPE_I8) or 448 (GLP_DTYPE_E4M3), so code * scale is the
  * value.  A row of zeros has codes 0 and scale 2^-100.  A row that holds a NaN or an infinity has
  * scale NaN, so that every value it stands for is NaN (codes unspecified). */
 typedef struct glp_norm_q8_args {

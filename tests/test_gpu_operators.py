@@ -147,6 +147,29 @@ def test_rounding_is_to_nearest_even():
     assert q.float().cpu().tolist() == [[448.0, 16.0, 20.0, 0.0, 2.0 ** -8, -16.0, 416.0, 448.0]]
 
 
+@pytest.mark.parametrize("qd", ["i8", "e4m3"])
+@pytest.mark.parametrize("h,pad", [(64, 0), (768, 0), (771, 0), (2048, 0), (1001, 3)])
+def test_exact_ties_of_16_bit_rows(h, pad, qd):
+    """f16 rows whose largest value is a power of two times `top`: every quotient v / scale is exact, many
+    fall halfway between two codes, and all must go to the even one."""
+    m = 64
+    g = torch.Generator(device="cuda")
+    g.manual_seed(h)
+    v = torch.randint(-254, 255, (m, h), generator=g, device="cuda").float() / 2  # halves, within +-127
+    if qd == "e4m3":
+        v = torch.round(v * 8) / 4  # quarters and coarser: ties of every binade
+    top = TOP[qd]
+    v = v.clamp(-top, top)
+    v[:, h // 2] = top
+    up = torch.arange(m, device="cuda")[:, None] % 5 - 2
+    x = filled(v * 2.0 ** up, "f32" if qd == "e4m3" else "f16", pad)
+    q, s = buffer(m, h, qd, pad), torch.empty(m, device="cuda")
+    run_quantize(x, q, s, "f32" if qd == "e4m3" else "f16", qd)
+    assert torch.equal(s, 2.0 ** up[:, 0].float())
+    want = torch.round(v) if qd == "i8" else v.to(torch.float8_e4m3fn).float()  # both to the even one
+    assert torch.equal(q.float(), want)
+
+
 # ------------------------------------------------------------------------------------- norm
 
 def norm_want(x, res, post, gain, scalar):
@@ -227,6 +250,19 @@ def test_norm_edge_rows(h):
     check_codes(q[clean], s[clean], n, "e4m3", n_mag)
     assert (q[0].float() == 0).all() and s[0] == FLOOR
     assert torch.isnan(q.float() * s[:, None])[[2, 3]].all()
+
+
+@pytest.mark.parametrize("qd", ["i8", "e4m3"])
+@pytest.mark.parametrize("h", [64, 77, 768, 2051])
+@pytest.mark.parametrize("eps", [1e-30, 1e-6, 1.0])
+def test_norm_zero_rows_whatever_the_eps(h, qd, eps):
+    x = torch.zeros((5, h), dtype=torch.float32, device="cuda")
+    x[1] = 1.0
+    q, s = buffer(5, h, qd), torch.empty(5, device="cuda")
+    api.norm_residual_q8(5, h, ptr(x), DT["f32"], ptr(q), DT[qd], ptr(s), h_dtype=DT["f32"], eps=eps)
+    rows = [0, 2, 3, 4]
+    assert (q[rows].float() == 0).all() and (s[rows] == FLOOR).all()
+    assert (q[1].float() == TOP[qd]).all()
 
 
 def test_rows_past_32_bit_offsets():
