@@ -45,17 +45,19 @@ __device__ __forceinline__ void mma_rows(typename RowsAcc<DT>::T (&d)[4], uint32
 #undef GLP_MMA
 }
 
-// 16 bytes at byte offset b of a row of `bytes` bytes, zeros past its end
+// 16 bytes at byte offset b of a row of `bytes` bytes, zeros past its end.  Coherent loads: under a dependent
+// launch this kernel is already resident while the one before it writes x (or w), so neither is read-only
+// for the kernel's life, which the non-coherent path asks for; volatile, so that none moves over the wait.
 template <bool STREAM>
 __device__ __forceinline__ uint4 load16(const uint8_t* row, int b, int bytes) {
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
   if (b + 16 <= bytes) {
     if constexpr (STREAM)
-      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+      v = ld_stream(row + b);
+    else
+      asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                    : "l"(row + b));
-    else
-      v = __ldg(reinterpret_cast<const uint4*>(row + b));
   } else if (b < bytes) {
     uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
