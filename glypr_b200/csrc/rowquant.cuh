@@ -202,6 +202,24 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {  // read once: no li
   return v;
 }
 
+// The gains: kept in L1, for every row reads them again, by coherent loads, for the kernel is resident while the
+// call before it may still write them.  Neither volatile nor tied to memory, so that they are free to move up
+// among the row's loads and stores; only the pointers, made after the wait, hold them behind it.
+__device__ __forceinline__ const float* after_wait(const float* p) {
+  asm volatile("" : "+l"(p) : : "memory");
+  return p;
+}
+__device__ __forceinline__ float4 ld_gain4(const float* p) {
+  float4 v;
+  asm("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float ld_gain(const float* p) {
+  float v;
+  asm("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
 // elements [e, e + 8) of the row at `row`, zeros for no chunk
 template <int DT>
 __device__ __forceinline__ Chunk<DT> load_chunk(const uint8_t* row, int e, bool on) {
@@ -302,23 +320,22 @@ __device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int
   }
   const int s = SHIFTED ? e & 3 : 0;
   if (!SHIFTED || (aligned16 && s == 0)) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(gain + e)), b = __ldg(reinterpret_cast<const float4*>(gain + e) + 1);
+    const float4 a = ld_gain4(gain + e), b = ld_gain4(gain + e + 4);
     p[0] = f2(a.x, a.y), p[1] = f2(a.z, a.w), p[2] = f2(b.x, b.y), p[3] = f2(b.z, b.w);
     return;
   }
   float v[8];
   if (aligned16) {
     float w[12];
-    const float4* at = reinterpret_cast<const float4*>(gain + (e - s));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float4 f = __ldg(at + i);
+      const float4 f = ld_gain4(gain + (e - s) + 4 * i);
       w[4 * i] = f.x, w[4 * i + 1] = f.y, w[4 * i + 2] = f.z, w[4 * i + 3] = f.w;
     }
     // (the s values that the third word is needed for; the row may end with them)
-    w[8] = __ldg(gain + (e - s + 8));
-    w[9] = s > 1 ? __ldg(gain + (e - s + 9)) : 0.0f;
-    w[10] = s > 2 ? __ldg(gain + (e - s + 10)) : 0.0f;
+    w[8] = ld_gain(gain + (e - s + 8));
+    w[9] = s > 1 ? ld_gain(gain + (e - s + 9)) : 0.0f;
+    w[10] = s > 2 ? ld_gain(gain + (e - s + 10)) : 0.0f;
     w[11] = 0.0f;
     // a shift by s in two steps, so that every index is known at compile time
 #pragma unroll
@@ -327,7 +344,7 @@ __device__ __forceinline__ void load_gain(const float* gain, bool aligned16, int
     for (int j = 0; j < 8; ++j) v[j] = s & 1 ? w[j + 1] : w[j];
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __ldg(gain + e + j);
+    for (int j = 0; j < 8; ++j) v[j] = ld_gain(gain + e + j);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) p[j] = f2(v[2 * j], v[2 * j + 1]);
@@ -345,8 +362,12 @@ constexpr int kShifted = 0, kFlush = 1, kFull = 2;
 
 // G threads per row, NC chunks per thread: a row has at most G NC whole chunks.  XT, HT: types of x and of
 // residual / h.  gains16: both gains start on 16-byte boundaries (kFlush and kFull promise it).
+// A norm of 5 chunks a lane in 16-bit types needs just over the 80 registers that three blocks per SM leave
+// (65,536 x 1,152, both norms: 101 us, 121 us with two).
+template <int G, int NC, int XT, int HT, bool NORM>
+constexpr int kRowBlocks = NORM && G == 32 && NC == 5 && kBytes<XT> == 2 && kBytes<HT> == 2 ? 3 : 0;
 template <int G, int NC, int XT, int HT, bool NORM, int PLACE>
-__global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQuantParams p, bool gains16) {
+__global__ void __launch_bounds__(G <= 32 ? 256 : G, kRowBlocks<G, NC, XT, HT, NORM>) row_quant_kernel(const RowQuantParams p, bool gains16) {
   constexpr int ROWS = G <= 32 ? 256 / G : 1;
   constexpr bool SHIFTED = PLACE == kShifted;
   constexpr int ED = !SHIFTED ? 0 : (G >= 16 ? 1 : 2);  // head and tail elements per lane
@@ -383,6 +404,7 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
   uint64_t v[NC][4];
   float none = 0.0f, amax = 0.0f;
   if constexpr (NORM) {
+    const float *post_gain = after_wait(p.post_gain), *gain = after_wait(p.gain);
     const uint8_t* rr = static_cast<const uint8_t*>(p.residual) + row * p.ld_residual * kBytes<HT>;
     uint8_t* hr = static_cast<uint8_t*>(p.h) + row * p.ld_h * kBytes<HT>;
     Chunk<HT> rc[NC];
@@ -407,7 +429,7 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
 #pragma unroll
     for (int c = 0; c < NC; ++c) chunk_f32<XT>(xc[c], v[c]);
     uint64_t inv2 = f2(1.0f, 1.0f);
-    if (p.post_gain) {
+    if (post_gain) {
       uint64_t ss2 = f2(0.0f, 0.0f);
 #pragma unroll
       for (int c = 0; c < NC; ++c)
@@ -420,7 +442,7 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
       const float inv = inv_rms(ss, p);
       inv2 = f2(inv, inv);
 #pragma unroll
-      for (int d = 0; d < ED; ++d) ve[d] = ve[d] * inv * (oe[d] ? __ldg(p.post_gain + ne[d]) : 0.0f);
+      for (int d = 0; d < ED; ++d) ve[d] = ve[d] * inv * (oe[d] ? ld_gain(post_gain + ne[d]) : 0.0f);
     }
     const uint64_t scalar2 = f2(p.layer_scalar, p.layer_scalar);
     uint64_t ss2 = f2(0.0f, 0.0f);
@@ -428,8 +450,8 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
     for (int c = 0; c < NC; ++c) {
       const int e = e_of(c);
       uint64_t g[4];
-      if (p.post_gain) {
-        load_gain<SHIFTED>(p.post_gain, gains16, e, on(c), g);
+      if (post_gain) {
+        load_gain<SHIFTED>(post_gain, gains16, e, on(c), g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(f2_mul(v[c][j], inv2), g[j]);
       }
@@ -445,8 +467,8 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
         ss2 = f2_fma(v[c][j], v[c][j], ss2);
       }
       if (p.h) store_chunk<HT>(hr, e, on(c), v[c]);
-      if (p.gain) {
-        load_gain<SHIFTED>(p.gain, gains16, e, on(c), g);
+      if (gain) {
+        load_gain<SHIFTED>(gain, gains16, e, on(c), g);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[c][j] = f2_mul(v[c][j], g[j]);
       }
@@ -459,7 +481,7 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G) row_quant_kernel(const RowQ
       ve[d] *= p.layer_scalar;
       ss = fmaf(ve[d], ve[d], ss);
       if (p.h && oe[d]) store_from_f32(hr, ne[d], HT, ve[d]);
-      if (p.gain) ve[d] *= oe[d] ? __ldg(p.gain + ne[d]) : 0.0f;
+      if (gain) ve[d] *= oe[d] ? ld_gain(gain + ne[d]) : 0.0f;
       amax = max_nan(amax, fabsf(ve[d]));
     }
     row_reduce<G, true, true>(ss, amax);

@@ -113,3 +113,37 @@ def test_products_in_a_chain(m):
         between()
     assert ROUNDS % 2 == 0
     eager_and_graph(step, bufs[0])
+
+
+@pytest.mark.parametrize("h", [64, 768, 771, 1152, 2051, 9000])
+def test_norm_with_gains_just_written(h):
+    """Both gains are rows that the product before the norm wrote, new ones each time."""
+    m, k = 40, 16
+    src = randn(h, ROUNDS, 2, k).half()
+    w = (randn(h + 1, h, k) / 4).half()
+    x, res = randn(h + 2, m, h).half(), randn(h + 3, m, h).bfloat16()
+    pitch = (h + 3) // 4 * 4
+    gains = torch.empty((2, pitch), device="cuda")
+    q, s = torch.empty((ROUNDS, m, h), dtype=torch.int8, device="cuda"), torch.empty((ROUNDS, m), device="cuda")
+    hout = torch.empty((m, h), dtype=torch.bfloat16, device="cuda")
+    outs = torch.empty((ROUNDS, m, h + 1), device="cuda")
+
+    def step(i, between):
+        api.linear(2, h, k, DT["f16"], src[i].data_ptr(), w.data_ptr(), gains.data_ptr(), DT["f32"], ldy=pitch, stream=stream())
+        between()
+        api.norm_residual_q8(m, h, x.data_ptr(), DT["f16"], q[i].data_ptr(), DT["i8"], s[i].data_ptr(),
+                             gain=gains[0].data_ptr(), post_gain=gains[1].data_ptr(), residual=res.data_ptr(),
+                             h=hout.data_ptr(), h_dtype=DT["bf16"], stream=stream())
+        between()
+        if i == ROUNDS - 1:
+            outs[:, :, :h].copy_(q)
+            outs[:, :, h].copy_(s)
+    eager_and_graph(step, outs)
+    # the last round's rows against the formula; int8 codes: half a step of 1 / 127 of the row's largest value
+    post, gain = ((src[-1, r].double() @ w.double().T) for r in (1, 0))
+
+    def rms(v):
+        return v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-6)
+    n = rms(res.double() + rms(x.double()) * post) * gain
+    err = (q[-1].double() * s[-1].double()[:, None] - n).abs()
+    assert (err <= 0.501 * n.abs().amax(1, keepdim=True) / 127).all()
