@@ -1,5 +1,7 @@
 // Host side of glp_norm_residual_q8 and glp_quantize_rows: argument checks, the choice of kernel,
 // launches.
+#include <algorithm>
+
 #include "op_rows.cuh"
 
 namespace {
@@ -53,7 +55,9 @@ int norm_residual_q8(const glp_norm_q8_args* a, cudaStream_t st) {
   p.x = a->x, p.residual = a->residual, p.post_gain = a->post_gain, p.gain = a->gain;
   p.h = a->h, p.q = a->q, p.scale = a->scale;
   p.ld_x = a->ld_x, p.ld_residual = a->ld_residual, p.ld_h = a->ld_h, p.ld_q = a->ld_q;
-  p.eps = a->eps, p.layer_scalar = a->layer_scalar, p.inv_H = static_cast<float>(1.0 / p.H);
+  // At least the smallest normal f32: a row of zeros then keeps its zeros, and what squares lose below f32's range
+  // is lost against it.
+  p.eps = std::max(a->eps, 1.17549435e-38f), p.layer_scalar = a->layer_scalar, p.inv_H = static_cast<float>(1.0 / p.H);
   p.x_dtype = a->x_dtype, p.h_dtype = a->h_dtype, p.q_dtype = a->q_dtype;
   if (!pitch(&p.ld_x, p.H) || !pitch(&p.ld_residual, p.H) || !pitch(&p.ld_h, p.H) || !pitch(&p.ld_q, p.H))
     return fail(GLP_ERR_INVALID_ARG, "a row pitch is shorter than H");

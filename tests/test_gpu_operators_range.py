@@ -1,0 +1,76 @@
+"""The row operators at the ends of f32's range: rows of zeros without an eps, rows whose squares f32 cannot hold,
+rows smaller than a quotient by them."""
+from __future__ import annotations
+
+import pytest
+
+from glypr_b200 import api
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DT = api.DTYPES
+TORCH = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i8": torch.int8,
+         "e4m3": torch.float8_e4m3fn}
+TOP = {"i8": 127.0, "e4m3": 448.0}
+FLOOR = 2.0 ** -100
+# widths of every form: 8 lanes to 1,024 threads per row, whole lanes, off chunk boundaries
+WIDTHS = [8, 64, 77, 256, 512, 768, 771, 1152, 1543, 2048, 5000, 12000, 20001]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    api.load_library()
+    yield
+
+
+def ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def randn(seed, *shape):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def norm(x, qd, eps, post=None, res=None, gain=None, apart=False):
+    """(codes as f32, scale, h); apart: q off x's place in its chunks of 8, which takes the kernel for any
+    alignment."""
+    m, h = x.shape
+    hout = torch.full_like(x, float("nan"))
+    flat = torch.zeros(m * h + 16, dtype=torch.int8, device="cuda")
+    q = flat[1 if apart else 0:][:m * h].view(m, h).view(TORCH[qd])
+    s = torch.empty(m, device="cuda")
+    xd = next(k for k, t in TORCH.items() if t == x.dtype)
+    api.norm_residual_q8(m, h, ptr(x), DT[xd], ptr(q), DT[qd], ptr(s), gain=ptr(gain), post_gain=ptr(post),
+                         residual=ptr(res), h=ptr(hout), h_dtype=DT[xd], eps=eps)
+    return q.float(), s, hout
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("qd", ["i8", "e4m3"])
+@pytest.mark.parametrize("h", WIDTHS)
+def test_zero_rows_without_an_eps(h, qd, apart):
+    """Codes 0 and the smallest scale, as for any other eps; the rows beside them are as ever."""
+    x = randn(h, 6, h).bfloat16()
+    x[1] = 0
+    x[4] = 0
+    post = randn(h + 1, h).abs() + 0.5
+    for p in (None, post):
+        q, s, hout = norm(x, qd, 0.0, post=p, apart=apart)
+        q1, s1, h1 = norm(x, qd, 1e-30, post=p, apart=apart)
+        assert (q[[1, 4]] == 0).all() and (s[[1, 4]] == FLOOR).all() and (hout[[1, 4]] == 0).all()
+        assert torch.equal(q, q1) and torch.equal(s, s1) and torch.equal(hout, h1)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("h", WIDTHS)
+def test_small_rows_without_an_eps(h, apart):
+    """Rows of 1e-15 (squares of 1e-30) have the norm of the same rows times 2^50."""
+    x = randn(h, 5, h) * 1e-15
+    q, s, _ = norm(x, "i8", 0.0, apart=apart)
+    q1, s1, _ = norm(x * 2.0 ** 50, "i8", 0.0, apart=apart)
+    # the squares' sum and eps = 2^-126 against 1e-30: the statistic to 2^-22, codes apart by one step at most
+    assert ((s / s1 - 1).abs() <= 2.0 ** -20).all()
+    assert ((q - q1).abs() <= 1).all() and (q != q1).float().mean() < 1e-3
