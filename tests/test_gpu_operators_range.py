@@ -74,3 +74,31 @@ def test_small_rows_without_an_eps(h, apart):
     # the squares' sum and eps = 2^-126 against 1e-30: the statistic to 2^-22, codes apart by one step at most
     assert ((s / s1 - 1).abs() <= 2.0 ** -20).all()
     assert ((q - q1).abs() <= 1).all() and (q != q1).float().mean() < 1e-3
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dtype,qd", [("f32", "i8"), ("bf16", "e4m3")])
+@pytest.mark.parametrize("h", WIDTHS)
+def test_rows_whose_squares_overflow(h, dtype, qd, apart):
+    """Finite rows of 2^70: no zeros in place of their norm, but a scale of NaN; the rows beside them as ever."""
+    x = randn(h, 6, h)
+    x[2] *= 2.0 ** 70
+    x[5, h // 2] = 2.0 ** 100
+    x = x.to(TORCH[dtype])
+    clean, big = [0, 1, 3, 4], [2, 5]
+    post, res = randn(h + 1, h).abs() + 0.5, randn(h + 2, 6, h).to(TORCH[dtype])
+    for p in (None, post):
+        q, s, hout = norm(x, qd, 1e-6, post=p, res=res, apart=apart)
+        assert torch.isnan(s[big]).all() and torch.isfinite(s[clean]).all()
+        assert torch.isnan(q[big] * s[big, None]).all()
+        assert torch.isfinite(hout[clean]).all()
+        if p is None:
+            assert torch.equal(hout, (x.float() + res.float()).to(x.dtype))
+        q1, s1, h1 = norm(x[clean].contiguous(), qd, 1e-6, post=p, res=res[clean].contiguous(), apart=apart)
+        if h % 8 == 0 or apart:  # (else the rows' places, and so the order of their sums, differ)
+            assert torch.equal(q[clean], q1) and torch.equal(s[clean], s1)
+    # up to there the norm is the norm
+    y = randn(h, 3, h) * 2.0 ** 55
+    q, s, _ = norm(y, "i8", 1e-6, apart=apart)
+    q1, s1, _ = norm(y * 2.0 ** -55, "i8", 0.0, apart=apart)
+    assert torch.equal(q, q1) and ((s / s1 - 1).abs() <= 2.0 ** -22).all()
