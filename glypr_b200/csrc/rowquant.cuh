@@ -115,10 +115,13 @@ __device__ __forceinline__ float inv_rms(float ss, const RowQuantParams& p) {
 // The factor from values to codes: top / amax by one rounded quotient (the rms and the scale's own rounding
 // cancel in it), and 1 / scale where the scale is the floor.  With the quotient of the rounded rms and scale
 // in its place three times as many codes fell on the other side of a rounding boundary.
-__device__ __forceinline__ float code_factor(float amax, float inv, float s, int q_dtype) {
+__device__ __forceinline__ float code_factor(float amax, float inv, float& s, int q_dtype) {
   const bool above = s > kQuantFloor;  // (a scale of NaN: whatever the code)
-  // finite, so that zeros keep code 0 also where eps is so small that 1 / (rms scale) overflows
-  return fminf((above ? quant_top(q_dtype) : inv) / (above ? amax : s), 3.4028235e38f);
+  const float k = (above ? quant_top(q_dtype) : inv) / (above ? amax : s);
+  // No codes where top / amax is beyond f32 (|h gain| under 2^-118 through an eps under 1e-15), rather than
+  // ones of another row; and a finite factor, so that zeros keep code 0 where 1 / (rms scale) overflows.
+  if (above && k > kMaxF32) s = __int_as_float(0x7fffffff);
+  return fminf(k, kMaxF32);
 }
 
 // One element at a time, any alignment: G threads per row, NC elements per thread, H <= G * NC.
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(G < 128 ? 128 : G) row_quant_any_kernel(const 
     }
     row_reduce<G>(ss, amax);
     const float inv_h = inv_rms(ss, p);
-    const float s = scale_of(amax * inv_h, p.q_dtype);
+    float s = scale_of(amax * inv_h, p.q_dtype);
     const float k = code_factor(amax, inv_h, s, p.q_dtype);
     if (t == 0) p.scale[row] = s;
 #pragma unroll
@@ -493,7 +496,7 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G, kRowBlocks<G, NC, XT, HT, N
     }
     row_reduce<G, true, true>(ss, amax);
     const float inv_h = inv_rms(ss, p);
-    const float s = scale_of(amax * inv_h, p.q_dtype);
+    float s = scale_of(amax * inv_h, p.q_dtype);
     const float k = code_factor(amax, inv_h, s, p.q_dtype);
     if (t == 0) p.scale[row] = s;
 #pragma unroll

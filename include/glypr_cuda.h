@@ -385,9 +385,10 @@ typedef struct glp_norm_q8_args {
  *   x~ = x * rms(x) * post_gain (or x),  h = (residual + x~) * layer_scalar,
  *   (q, scale) = 8-bit form of h * rms(h) * gain,   rms(v) = 1 / sqrt(mean(v^2) + eps),
  * eps >= 0 and taken as at least 2^-126 (so a row of zeros gives zeros), all in f32: a row of x with a
- * post_gain, or of h, whose sum of squares f32 cannot hold counts as one that holds an infinity.  h is rounded
- * once, to h_dtype, and the norm continues from the unrounded value (as the model path's
- * post_norm_residual does; norm.rs:22-94, layer.rs:20-50). */
+ * post_gain, or of h, whose sum of squares f32 cannot hold counts as one that holds an infinity, and so does
+ * one of |h * gain| under 2^-118 whose norm is not that small.  h is rounded once, to h_dtype, and the norm
+ * continues from the unrounded value (as the model path's post_norm_residual does; norm.rs:22-94,
+ * layer.rs:20-50). */
 int glp_norm_residual_q8(const glp_norm_q8_args* args, void* stream);
 
 /* q, scale [M] = the 8-bit form of each row of x [M, H] (F32 / F16 / BF16): weights once at load,

@@ -102,3 +102,22 @@ def test_rows_whose_squares_overflow(h, dtype, qd, apart):
     q, s, _ = norm(y, "i8", 1e-6, apart=apart)
     q1, s1, _ = norm(y * 2.0 ** -55, "i8", 0.0, apart=apart)
     assert torch.equal(q, q1) and ((s / s1 - 1).abs() <= 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("qd", ["i8", "e4m3"])
+@pytest.mark.parametrize("h", WIDTHS)
+def test_rows_below_the_factor_of_their_codes(h, qd, apart):
+    """Codes and scales stand for the row's norm, or the scale is NaN: no other values.  Gains of 2^-75 let a
+    row of ordinary size come that near to zero, an eps of 0 one that is small itself."""
+    x = randn(h, 8, h) * 2.0 ** torch.tensor([-40.0, -44, -48, -52, -55, -58, -60, -62], device="cuda")[:, None]
+    gain = torch.full((h,), 2.0 ** -72, device="cuda")
+    q, s, _ = norm(x, qd, 0.0, gain=gain, apart=apart)
+    # the norm of x in 64 bits, its gain left out: 2^-72 of it is far above the smallest scale
+    n = x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True) + 2.0 ** -126)
+    v = q.double() * s.double()[:, None] * 2.0 ** 72
+    top = n.abs().amax(1, keepdim=True)
+    step = 1 / 127 if qd == "i8" else 1 / 14  # e4m3: 2^-3 of a binade, of 448 at most 32
+    fine = torch.isnan(s)[:, None] | ((v - n).abs() <= 0.51 * step * top)
+    assert fine.all()
+    assert torch.isfinite(s[:2]).all()  # |h gain| of 2^-112 and 2^-116 have their codes
