@@ -79,13 +79,16 @@ __global__ void __launch_bounds__(256) linear_any_kernel(const LinearParams p) {
       for (int j = 0; j < 4; ++j) {
         const int64_t n = n0 + tx + 16 * j;
         if (n >= p.N) continue;
-        float v = static_cast<float>(acc[i][j]) * (p.w_scale ? xs * p.w_scale[n] : xs);
+        // (the sum first: the two scales' own product may leave f32's range where the value does not)
+        float v = static_cast<float>(acc[i][j]) * xs;
+        if (p.w_scale) v *= p.w_scale[n];
         if (p.bias) v += p.bias[n];
         float pair[2] = {v, v};
         activate_all(pair, p.activation);
         v = pair[0];
         if constexpr (GATED) {
-          float u = static_cast<float>(up[i][j]) * (p.w_up_scale ? xs * p.w_up_scale[n] : xs);
+          float u = static_cast<float>(up[i][j]) * xs;
+          if (p.w_up_scale) u *= p.w_up_scale[n];
           if (p.bias_up) u += p.bias_up[n];
           v *= u;
         }

@@ -121,3 +121,40 @@ def test_rows_below_the_factor_of_their_codes(h, qd, apart):
     fine = torch.isnan(s)[:, None] | ((v - n).abs() <= 0.51 * step * top)
     assert fine.all()
     assert torch.isfinite(s[:2]).all()  # |h gain| of 2^-112 and 2^-116 have their codes
+
+
+@pytest.mark.parametrize("off", [0, 3])
+@pytest.mark.parametrize("m", [4, 40, 200])
+@pytest.mark.parametrize("gated", [False, True])
+def test_scales_whose_product_leaves_the_range(m, gated, off):
+    """x_scale * w_scale of 1e-42 and of 1e42, with sums that bring the value back: operands on and off 16-byte
+    rows."""
+    n, k = 72, 96
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+
+    def codes(rows):
+        flat = torch.zeros(rows * k + 16, dtype=torch.int8, device="cuda")
+        v = flat[off:off + rows * k].view(rows, k)
+        v.copy_(torch.randint(-127, 128, (rows, k), generator=g, device="cuda"))
+        return v
+    x, w, wu = codes(m), codes(n), codes(n)
+    x[1] = 0  # sums of 0: 0 whatever the scales
+    for sx, sw in ((1e-30, 1e-12), (1e22, 1e20)):
+        xs, ws = torch.full((m,), sx, device="cuda"), torch.full((n,), sw, device="cuda")
+        one = torch.full((n,), 1 / sx, device="cuda")  # the gate's scales undone
+        if sx > 1:
+            x[2:] = 0
+        y = torch.full((m, n), float("nan"), device="cuda")
+        up = dict(w_up=wu.data_ptr(), w_up_scale=one.data_ptr()) if gated else {}
+        api.linear(m, n, k, DT["i8"], x.data_ptr(), w.data_ptr(), y.data_ptr(), DT["f32"], x_scale=xs.data_ptr(),
+                   w_scale=ws.data_ptr(), activation=api.ACTIVATIONS["none"], **up)
+        rows = slice(None) if sx < 1 else slice(1, None)
+        want = (x.double() @ w.double().T) * xs.double()[:, None] * ws.double()
+        u = torch.ones_like(want)
+        if gated:
+            u = (x.double() @ wu.double().T) * xs.double()[:, None] * one.double()
+        want = want * u
+        # three products of f32 for each factor, on sums that f32 holds exactly; the first may be subnormal
+        bound = 2.0 ** -21 * want.abs() + 2.0 ** -149 * (1 + u.abs())
+        assert ((y.double() - want).abs() <= bound)[rows].all()
