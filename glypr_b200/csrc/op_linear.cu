@@ -78,7 +78,7 @@ int raise_smem(K kernel, size_t smem, int dev, std::atomic<uint64_t>* ready) {
   const uint64_t bit = 1ull << dev;
   if (ready->load(std::memory_order_relaxed) & bit) return GLP_OK;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) return fail(GLP_ERR_CUDA, cudaGetErrorString(e));
+  if (e != cudaSuccess) return launched(e);
   ready->fetch_or(bit, std::memory_order_relaxed);
   return GLP_OK;
 }

@@ -28,8 +28,9 @@ inline int fail(int code, const char* msg) {
   return code;
 }
 
-inline int launched(cudaError_t e = cudaGetLastError()) {
+inline int launched(cudaError_t e) {
   if (e == cudaSuccess) return GLP_OK;
+  cudaGetLastError();  // reported here and not once more by the next call that asks for it
   set_last_error(std::string("kernel launch: ") + cudaGetErrorString(e));
   return e == cudaErrorMemoryAllocation ? GLP_ERR_OOM : GLP_ERR_CUDA;
 }
