@@ -213,8 +213,10 @@ int launch_rows(const LinearParams& p, const DeviceInfo& d, cudaStream_t st) {
   if (p.M <= 16)
     return p.N <= 16 * d.sms ? launch_rows<DT, GATED, 1, 1, 2, 16>(p, st) : launch_rows<DT, GATED, 1, 2, 2, 16>(p, st);
   if (p.M <= 32) {
-    if (GATED) return launch_rows<DT, GATED, 2, 1, 1, 16>(p, st);
-    return p.N <= 8 * d.sms ? launch_rows<DT, GATED, 2, 1, 2, 16>(p, st) : launch_rows<DT, GATED, 2, GATED ? 1 : 2, 1, 16>(p, st);
+    if constexpr (GATED)
+      return launch_rows<DT, true, 2, 1, 1, 16>(p, st);
+    else
+      return p.N <= 8 * d.sms ? launch_rows<DT, false, 2, 1, 2, 16>(p, st) : launch_rows<DT, false, 2, 2, 1, 16>(p, st);
   }
   return launch_rows<DT, GATED, 4, 1, 1, GATED ? 8 : 16>(p, st);  // gated: sums of 16 warps would not fit
 }
