@@ -7,7 +7,8 @@ Takes a layer's gate, up and down weights as a GGUF holds them (Q8_0 blocks; her
 glp_quantize_rows, once), and runs
 
     h, (q, s)  = glp_norm_residual_q8     h += post-norm of the attention block's output; pre-norm in int8
-    a          = glp_linear (gated)       gelu_tanh(q Wgate^T) * (q Wup^T), f16
+    a          = glp_linear (gated)       gelu_tanh(q Wgate^T) * (q Wup^T), f32: in f16 its
+                                          rounding would move codes, and 65,504 end it
     (qa, sa)   = glp_quantize_rows        a in int8
     y          = glp_linear               qa Wdown^T, f16: the input of the layer's next post-norm
 
@@ -42,7 +43,7 @@ class Int8FeedForward:
         self.gate, self.up, self.down = (self.quantized(w) for w in (gate, up, down))
         dev = gate.device
         self.q = torch.empty((max_tokens, self.h), dtype=torch.int8, device=dev)
-        self.a = torch.empty((max_tokens, self.f), dtype=torch.float16, device=dev)
+        self.a = torch.empty((max_tokens, self.f), device=dev)
         self.qa = torch.empty((max_tokens, self.f), dtype=torch.int8, device=dev)
         self.scales = torch.empty((2, max_tokens), device=dev)
 
@@ -63,10 +64,10 @@ class Int8FeedForward:
         api.norm_residual_q8(m, self.h, attn_out.data_ptr(), DT["f16"], self.q.data_ptr(), DT["i8"], s,
                              gain=self.gain.data_ptr(), post_gain=self.post_gain.data_ptr(),
                              residual=residual.data_ptr(), h=residual.data_ptr(), h_dtype=DT["bf16"], eps=EPS, stream=st)
-        api.linear(m, self.f, self.h, DT["i8"], self.q.data_ptr(), self.gate[0].data_ptr(), self.a.data_ptr(), DT["f16"],
+        api.linear(m, self.f, self.h, DT["i8"], self.q.data_ptr(), self.gate[0].data_ptr(), self.a.data_ptr(), DT["f32"],
                    x_scale=s, w_scale=self.gate[1].data_ptr(), w_up=self.up[0].data_ptr(),
                    w_up_scale=self.up[1].data_ptr(), activation=api.ACTIVATIONS["gelu_tanh"], stream=st)
-        api.quantize_rows(m, self.f, self.a.data_ptr(), DT["f16"], self.qa.data_ptr(), DT["i8"], sa, stream=st)
+        api.quantize_rows(m, self.f, self.a.data_ptr(), DT["f32"], self.qa.data_ptr(), DT["i8"], sa, stream=st)
         api.linear(m, self.h, self.f, DT["i8"], self.qa.data_ptr(), self.down[0].data_ptr(), y.data_ptr(), DT["f16"],
                    x_scale=sa, w_scale=self.down[1].data_ptr(), stream=st)
         return y
