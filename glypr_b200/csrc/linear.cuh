@@ -44,8 +44,9 @@ __device__ __forceinline__ float rcp_fast(float x) {
 //
 // erf-GELU is max(v, 0) - 0.5 |v| erfc(|v| / sqrt 2).  With x = |v| / sqrt 2 and t = 1 / (1 + x/2),
 // erfc(x) = t 2^(P(t - 0.6) - x^2 log2 e): log2(e^(x^2) erfc(x) / t) is smooth in t, and P is its
-// minimax polynomial of degree 7 for x <= 11 (fitted for this file; 9e-7 relative with f32 arithmetic,
-// in the tail too).  |v| is cut at 64, where erfc is 0, so that an infinity stays one.
+// minimax polynomial of degree 7 for x <= 11 (fitted for this file).  Relative error with f32 arithmetic: 1e-6 for
+// |v| <= 1, and from there that of an exponent of up to 120 in f32: 3e-6 for |v| of 5 to 8, 8.4e-6 in the far
+// tail.  |v| is cut at 64, where erfc is 0, so that an infinity stays one.
 __device__ __forceinline__ float act_relu(float v) { return v < 0.0f ? 0.0f : v; }  // a NaN stays
 
 __device__ __forceinline__ uint64_t act_sigmoid_like(uint64_t v, uint64_t x) {  // v / (1 + 2^x)

@@ -1,7 +1,8 @@
 // y = act(x w^T xs ws + b) [* (x w_up^T xs wus + bu)] + residual for operands of any alignment:
 // 64 x 64 output tiles, 256 threads of 4 x 4 outputs, 16 columns of K at a time through shared
-// memory, one element per load.  Products are f32 FMAs (int8: exact int32 sums), which bound it: 131,072 x
-// 768 x 1,152 bf16 9.1 ms (25 TFLOP/s), 235 us on the tensor cores with 16-byte rows.
+// memory, one element per load.  Products are f32 FMAs (int8: exact int32 sums), which bound it: 32,768 x 768 x
+// 1,153 bf16 with packed rows 3.7 ms (16 TFLOP/s), 96 us on the tensor cores with rows of 1,160; one row against
+// 4,096 x 4,097 bf16, where 64 blocks walk K each by itself, 367 us, 11.1 us with rows of 4,104.
 #pragma once
 #include "linear.cuh"
 

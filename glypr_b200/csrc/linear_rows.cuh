@@ -9,12 +9,13 @@
 // w_up), its warps take the 64-byte steps of K in turn, and their sums are added in warp order, so a
 // result does not depend on timing.
 //
-// Many short-lived warps beat few with long prefetch queues: with 16 warps a block and two steps in
-// flight each, one row against 4,096 x 4,096 f16 weights takes 7.3 us (4 warps with 8 steps ahead: 12.9
-// us; the tensor-memory kernel: 22 us), gated 2 x 1,152 x 768 bf16 2.5 us (7.2 us), 8,191 x 4,096 e4m3 9.7
-// us (16.2 us), in a CUDA graph and so without the host's launch time.  What bounds the large ones is the
-// weights' way from memory (33.5 MB: 5.2 us at 6.5 TB/s) and one launch; past 32 rows x itself, read again
-// by every block, is the larger stream.
+// Many short-lived warps beat few with long prefetch queues: with 16 warps a block and two steps in flight each,
+// one row against 4,096 x 4,096 f16 weights takes 6.1 us where they stay in L2 and 9.5 us from memory (4 warps with
+// 8 steps ahead: 12.9 us), gated 2 x 1,152 x 768 bf16 2.6 and 3.0 us, 3 x 8,191 x 4,096 e4m3 9.2 and 11.3 us, in a
+// CUDA graph and so without the host's launch time.  From memory the large ones read at 3.0 to 3.5 TB/s, about half
+// of the copy rate: what bounds them is latency, for each block drains its loads before its warps' sums are
+// joined, and there are more blocks than fit at once.  Past 32 rows x itself, read again by every block, is the
+// larger stream.
 #pragma once
 #include "common.cuh"
 #include "linear.cuh"

@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(LinearTcCfg<CG, BN, GATED, EPI>::THREADS, 1)
               const int slice0 = col0 + c - in_slice;
               tma_store_2d(&tm_y, box, slice0, wrow0);
               bulk_commit();
-              if (res_tma && c + CH < cols) {  // f32 rows of 64 columns take the box twice
+              if (res_tma && c + CH < cols) {  // one of the warp's further boxes: up to four of f32, two of 16 bits
                 bulk_wait_read_all();
                 mbar_arrive_expect_tx(rb, 32 * row_bytes);
                 tma_load_2d(box, &tm_r, rb, slice0 + slice_cols, wrow0);

