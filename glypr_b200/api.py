@@ -461,15 +461,22 @@ def qkv_norm_rope(d_w: int, n_q_heads: int, n_kv_heads: int, k: int, d_x: int, m
                                            ctypes.c_void_p(d_out), ctypes.c_void_p(stream)))
 
 
+def _does_not_fit():
+    return GlyprError(GLP_ERR_INVALID_ARG, "an argument does not fit its integer type of the C interface")
+
+
 def norm_residual_q8(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dtype: int, d_scale: int, *,
                      gain: int = 0, post_gain: int = 0, residual: int = 0, h: int = 0, h_dtype: int = DTYPES["bf16"],
                      eps: float = 1e-6, layer_scalar: float = 1.0, ld_x: int = 0, ld_residual: int = 0, ld_h: int = 0,
                      ld_q: int = 0, stream: int = 0) -> None:
     """glp_norm_residual_q8: h = (residual + x~) * layer_scalar and the 8-bit form of RMSNorm(h) * gain.
     Device pointers as ints (0 = not given), types from ``DTYPES``, pitches in elements (0 = packed)."""
-    rc = (_lib or load_library()).glp_norm_residual_q8(
-        _NORM_Q8_ARGS.pack(m, h_len, d_x, ld_x, residual, ld_residual, post_gain, gain, eps, layer_scalar, h, ld_h, d_q,
-                           ld_q, d_scale, x_dtype, h_dtype, q_dtype), stream)
+    try:
+        args = _NORM_Q8_ARGS.pack(m, h_len, d_x, ld_x, residual, ld_residual, post_gain, gain, eps, layer_scalar, h, ld_h,
+                                  d_q, ld_q, d_scale, x_dtype, h_dtype, q_dtype)
+    except (struct.error, OverflowError):
+        raise _does_not_fit() from None
+    rc = (_lib or load_library()).glp_norm_residual_q8(args, stream)
     if rc:
         check(rc)
 
@@ -477,6 +484,8 @@ def norm_residual_q8(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dty
 def quantize_rows(m: int, h_len: int, d_x: int, x_dtype: int, d_q: int, q_dtype: int, d_scale: int, *,
                   ld_x: int = 0, ld_q: int = 0, stream: int = 0) -> None:
     """glp_quantize_rows: the 8-bit form (codes and one scale per row) of x [m, h_len]."""
+    if not (-2 ** 31 <= m < 2 ** 31 and -2 ** 31 <= h_len < 2 ** 31):  # ctypes would take them modulo 2^32
+        raise _does_not_fit()
     rc = (_lib or load_library()).glp_quantize_rows(d_x, x_dtype, ld_x, m, h_len, d_q, q_dtype, ld_q, d_scale, stream)
     if rc:
         check(rc)
@@ -489,9 +498,12 @@ def linear(m: int, n: int, k: int, dtype: int, d_x: int, d_w: int, d_y: int, out
     """glp_linear: y = act(x w^T * scales + bias) [* (x w_up^T * scales + bias_up)] + residual.
     Device pointers as ints (0 = not given), types from ``DTYPES``, ``activation`` from
     ``ACTIVATIONS``, pitches in elements (0 = packed)."""
-    rc = (_lib or load_library()).glp_linear(
-        _LINEAR_ARGS.pack(m, n, k, dtype, d_x, ldx, d_w, w_up, ldw, x_scale, w_scale, w_up_scale, bias, bias_up, residual,
-                          ld_residual, d_y, ldy, out_dtype, activation), stream)
+    try:
+        args = _LINEAR_ARGS.pack(m, n, k, dtype, d_x, ldx, d_w, w_up, ldw, x_scale, w_scale, w_up_scale, bias, bias_up,
+                                 residual, ld_residual, d_y, ldy, out_dtype, activation)
+    except (struct.error, OverflowError):
+        raise _does_not_fit() from None
+    rc = (_lib or load_library()).glp_linear(args, stream)
     if rc:
         check(rc)
 
