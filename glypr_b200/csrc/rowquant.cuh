@@ -421,8 +421,9 @@ __global__ void __launch_bounds__(G <= 32 ? 256 : G, kRowBlocks<G, NC, XT, HT, N
     Chunk<HT> rc[NC];
     float re[ED ? ED : 1];
     // Full rows: x and residual side by side, for which the compiler takes more registers and keeps more in
-    // flight (131,072 x 512: 86 us, 95 us with x first); the other kinds, whose x is on its way by now, are
-    // slower with it (65,536 x 1,152: 115 us, 101 us).
+    // flight (98,304 x 1,024 f16 and bf16 133 us, 159 us with x first; 196,608 x 512 117 / 120; f32 rows would
+    // rather have x first, 243 / 223); the other kinds, whose x is on its way by now, are slower with it
+    // (65,536 x 1,152: 115 us, 101 us).
     if constexpr (PLACE == kFull) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
