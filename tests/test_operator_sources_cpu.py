@@ -16,7 +16,7 @@ def code(name):
         return re.sub(r"//[^\n]*|/\*.*?\*/", "", f.read(), flags=re.S)
 
 
-@pytest.mark.parametrize("name", ["linear_rows.cuh", "rowquant.cuh"])
+@pytest.mark.parametrize("name", ["linear_rows.cuh", "rowquant.cuh", "linear_any.cuh", "linear_tc.cuh", "linear_splitk.cuh"])
 def test_dependent_launches_read_coherently(name):
     """A kernel that starts while the one before it still writes its operands may not read them through the
     non-coherent path, which asks for data that nothing writes during the kernel's life."""
